@@ -509,6 +509,48 @@ int pf_pad_fwd(const float* src, long sb, long s1, long sm, long s2, float* dst,
                int n1p, int n2p, int C, void* stream);
 
 /* ------------------------------------------------------------------------------
+ * Operators in the caller's own element type (training as well as inference): x, weights and
+ * results are all `dtype`, sums and statistics fp32.  Lengths are elements.
+ * -------------------------------------------------------------------------- */
+enum { PF_FP32 = 0, PF_FP16 = 1, PF_BF16 = 2 };
+
+/* Table lookup (nn.Embedding with a factor; the token -> atom broadcast of the atom transformer,
+ * tt_bio/boltz2.py, and one-hot projections as gathers):
+ *   out[i, :] = scale * weight[t_i, :],   a row of zeros where t_i is outside [0, V).
+ * index: int32 (index64 = 0) or int64 [n]; weight [V] rows of C, ldw elements apart; out [n][C]. */
+int pf_embedding_fwd(const void* index, int index64, const void* weight, long ldw, void* out, long n, long V, long C,
+                     int dtype, float scale, void* stream);
+
+/* Its gradient, and the atom -> token sum:  dw[v, :] = scale * sum over i with t_i = v of grad[i, :]
+ * (fp32, rounded once; zeros for rows that no token names).  grad [n][C]; dw [V][C], every row
+ * written.  The tokens are sorted with their positions first; no float atomics, so a call's bits
+ * depend on its inputs alone. */
+size_t pf_embedding_grad_workspace_size(long n, long V, long C);
+int pf_embedding_grad(const void* index, int index64, const void* grad, void* dw, long n, long V, long C, int dtype,
+                      float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Residual dropout (get_dropout_mask, tt_bio/boltz2.py:293-304, in z + mask * update,
+ * tt_bio/reference.py:877-903):
+ *   out[e] = residual[e] + (word(g(e)) >= rint(p 2^32) ? x[e] / (1 - p) : 0)
+ * on contiguous [B][I][J][C]; word(g) = word g % 4 of Philox4x32-10 at counter (g / 4, offset)
+ * under key `seed`.  g(e) = e (PF_DROP_ELEMENT), b I + i (PF_DROP_ROW) or b J + j
+ * (PF_DROP_COLUMN).  Dropped x are not used (a NaN there does not spread).  The gradient of x is
+ * the same call on the gradient, without residual.  out must not overlap x or residual. */
+enum { PF_DROP_ELEMENT = 0, PF_DROP_ROW = 1, PF_DROP_COLUMN = 2 };
+typedef struct pf_dropout_args {
+  long B, I, J, C;
+  int dtype, shared;
+  double p;
+  unsigned long long seed, offset;
+  const void* seed_at;    /* NULL, or a 64-bit seed in device memory, read when the kernel runs */
+  const void* x;
+  const void* residual;   /* or NULL: 0 */
+  void* out;
+  void* stream;
+} pf_dropout_args;
+int pf_dropout_add_fwd(const pf_dropout_args* args);
+
+/* ------------------------------------------------------------------------------
  * Measurement aids (no counterpart in the reference: they serve the benchmark's roofline
  * figures and allocate no device memory).
  * -------------------------------------------------------------------------- */

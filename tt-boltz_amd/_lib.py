@@ -124,6 +124,14 @@ class TransitionMx8Args(ctypes.Structure):
     ]
 
 
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_long), ("I", c_long), ("J", c_long), ("C", c_long), ("dtype", c_int), ("shared", c_int),
+        ("p", ctypes.c_double), ("seed", ctypes.c_ulonglong), ("offset", ctypes.c_ulonglong),
+        ("seed_at", c_void_p), ("x", c_void_p), ("residual", c_void_p), ("out", c_void_p), ("stream", c_void_p),
+    ]
+
+
 #: name -> (restype, argtypes); every symbol include/pairformer_hip.h declares.
 SIGNATURES = {
     "pf_abi_version": (c_int, []),
@@ -176,6 +184,12 @@ SIGNATURES = {
     "pf_trimul_mx8_contract": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "pf_transition_mx8_fwd": (c_int, [ctypes.POINTER(TransitionMx8Args)]),
     "pf_transition_mx8_pair_bias_fwd": (c_int, [ctypes.POINTER(TransitionMx8Args), ctypes.POINTER(ApbArgs)]),
+    "pf_embedding_fwd": (c_int, [c_void_p, c_int, c_void_p, c_long, c_void_p, c_long, c_long, c_long, c_int, c_float,
+                                 c_void_p]),
+    "pf_embedding_grad_workspace_size": (c_size_t, [c_long, c_long, c_long]),
+    "pf_embedding_grad": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_long, c_long, c_long, c_int, c_float, c_void_p,
+                                  c_size_t, c_void_p]),
+    "pf_dropout_add_fwd": (c_int, [ctypes.POINTER(DropoutArgs)]),
     "pf_attend_timing": (c_int, [c_int]),
     "pf_attend_timing_read": (c_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_int)]),
     "pf_kernel_timing": (c_int, [c_int, c_int]),

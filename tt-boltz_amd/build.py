@@ -19,6 +19,8 @@ OBJDIR = os.path.join(HERE, "_build")
 
 SOURCES = ["api.cpp", "trimul.hip", "triatt.hip", "transition.hip", "single.hip", "fast8.hip", "msa.hip", "diffusion.hip",
            "pad.hip", "measure.hip"]
+#: sources that work in the caller's element type: compiled once, linked into every library
+COMMON_SOURCES = ["embed.hip", "dropout.hip"]
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -53,9 +55,11 @@ def build(verbose: bool = True) -> list:
         objdir = os.path.join(OBJDIR, os.path.splitext(lib)[0])
         os.makedirs(objdir, exist_ok=True)
         jobs.append([(src, defines, objdir) for src in SOURCES])
+    jobs.append([(src, [], OBJDIR) for src in COMMON_SOURCES])
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
-        objs = [list(ex.map(_compile, j)) for j in jobs]
+        *objs, common = [list(c) for c in [ex.map(_compile, j) for j in jobs]]
     for (lib, _), o in zip(VARIANTS.items(), objs):
+        o = o + common
         path = os.path.join(HERE, lib)
         tmp = path + ".tmp"
         r = subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *o, "-o", tmp],

@@ -795,3 +795,10 @@ def launch_msa_embed(msa: torch.Tensor, has_deletion: Optional[torch.Tensor], de
     _lib.check(_lib.load(variant).pf_msa_embed(_ptr(msa), _ptr(has_deletion), _ptr(deletion_value), _ptr(msa_paired),
                                                _ptr(s_emb), _ptr(w_t), _ptr(m), B, S, N, m.shape[-1],
                                                w_t.shape[0] - 3, _stream()), "pf_msa_embed", variant)
+
+
+# operators between tracks, in the caller's own element type
+from .track_ops import (  # noqa: E402,F401
+    dropout_add, embedding, embedding_grad, embedding_grad_workspace_bytes, launch_dropout_add, launch_embedding,
+    launch_embedding_grad,
+)
