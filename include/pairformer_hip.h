@@ -550,6 +550,50 @@ typedef struct pf_dropout_args {
 } pf_dropout_args;
 int pf_dropout_add_fwd(const pf_dropout_args* args);
 
+/* Attention of one track's queries over another track's keys and values (the atom transformer's
+ * windows of 32 queries against 128 keys, tt_bio/boltz2.py AttentionPairBias with to_keys; tokens
+ * against atoms; a decoder against an encoder):
+ *   x_ij = scale q_i . k_j + bias_ij;  P = softmax over the keys that are seen;  o_i = sum_j P_ij v_j.
+ * q [B][Lq][H][D] and k, v [B][Lk][Hk][D] in `dtype`, any strides that are multiples of 16 bytes with
+ * contiguous channels; D a multiple of 8 up to 128; H / Hk heads share a key head.  Key j of batch
+ * element b is seen where j < k_lens[b] (clamped to [0, Lk]) and mask[b][j] != 0 (either may be
+ * NULL).  Hidden keys are not used, whatever stands there; a query that sees nothing (no key, or a
+ * bias of -inf throughout) has o = 0 and no gradient.  bias: any strides, fp32 or dtype.
+ * Scores, softmax and sums are fp32; P (16-bit types) is rounded to dtype for the product with v.
+ * For the backward pass, the forward pass keeps stats [2][B][H][Lq] (each row's maximum, and log2 of
+ * its sum) and, of 16-bit types, o32, the unrounded o: do_i . o_i loses its meaning next to
+ * do_i . v_j where one key has nearly all the weight if o is rounded first.  (With a bias gradient,
+ * 16-bit types form sum_j P_ij do_i . v_j instead, and o32 is not read.) */
+typedef struct pf_cross_attn_args {
+  int B, Lq, Lk, H, Hk, D;
+  int dtype, bias_dtype;
+  float scale;
+  const void* q; long q_b, q_l, q_h;
+  const void* k; long k_b, k_l, k_h;
+  const void* v; long v_b, v_l, v_h;
+  const void* bias; long bias_b, bias_h, bias_q, bias_k;   /* NULL: none */
+  const unsigned char* mask; long mask_b;                  /* [B] rows of Lk bytes, or NULL */
+  const int* k_lens;                                       /* [B], or NULL */
+  void* o;                /* [B][Lq][H][D] */
+  float* o32;             /* the same in fp32, or NULL */
+  float* stats;           /* [2][B][H][Lq], or NULL */
+  void* workspace; size_t workspace_bytes;
+  void* stream;
+  /* pf_cross_attn_bwd: gradients, contiguous; dq NULL: not wanted (dbias neither), dk and dv NULL:
+   * not wanted.  dbias [dbias_B][dbias_H][Lq][Lk] in bias_dtype, dbias_B 1 or B, dbias_H 1 or H: the
+   * sum over a dimension of size 1 (dbias_B = 0 and dbias NULL: not wanted). */
+  const void* dout;       /* [B][Lq][H][D] */
+  void* dq; void* dk; void* dv; void* dbias;
+  int dbias_B, dbias_H;
+} pf_cross_attn_args;
+
+size_t pf_cross_attn_workspace_size(const pf_cross_attn_args* args);
+int pf_cross_attn_fwd(const pf_cross_attn_args* args);
+/* The forward call's arguments and results (o of fp32, o32 of 16-bit types, stats) with the gradient
+ * fields.  No float atomics: a call's bits depend on its inputs alone. */
+size_t pf_cross_attn_bwd_workspace_size(const pf_cross_attn_args* args);
+int pf_cross_attn_bwd(const pf_cross_attn_args* args);
+
 /* ------------------------------------------------------------------------------
  * Measurement aids (no counterpart in the reference: they serve the benchmark's roofline
  * figures and allocate no device memory).

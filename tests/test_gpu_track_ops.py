@@ -135,6 +135,12 @@ def test_embedding_autograd(gpu, dtype):
     assert torch.equal(wd.grad, ops.embedding_grad(do.to(gpu), t.to(gpu), 50, 2.0))
     with torch.no_grad():
         assert not ops.embedding(t.to(gpu), wd).requires_grad
+    # the sum by token is a lookup's transpose, and the other way round
+    dod, dw = do.to(gpu).requires_grad_(), normal(g, 50, 40, dtype=dtype).to(gpu)
+    got, = torch.autograd.grad(ops.embedding_grad(dod, t.to(gpu), 50, 2.0), dod, dw)
+    assert torch.equal(got, ops.embedding(t.to(gpu), dw, 2.0))
+    first, = torch.autograd.grad(ops.embedding(t.to(gpu), wd, 2.0), wd, dod, create_graph=True)
+    assert torch.equal(torch.autograd.grad(first, dod, dw)[0], got)
 
 
 def test_embedding_grad_by_differences(gpu):
@@ -268,3 +274,369 @@ def test_two_streams_at_once(gpu):
                 got.append(ops.embedding_grad(do, t, 500))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
+
+
+# ------------------------------------------------------------------------------ cross attention
+def inputs(seed, dtype, B, Lq, Lk, H, Hk, D, bias=None, hide=None, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    c = {"q": normal(g, B, Lq, H, D, dtype=dtype, scale=scale), "k": normal(g, B, Lk, Hk, D, dtype=dtype),
+         "v": normal(g, B, Lk, Hk, D, dtype=dtype), "bias": None, "mask": None, "k_lens": None}
+    do = normal(g, B, Lq, H, D, dtype=dtype)
+    if bias:
+        bdt = dtype if "own" in bias else torch.float32
+        c["bias"] = normal(g, 1 if "b1" in bias else B, 1 if "h1" in bias else H, Lq, Lk, dtype=bdt)
+    if hide in ("mask", "both"):
+        c["mask"] = torch.rand((B, Lk), generator=g) < 0.7
+    if hide in ("lens", "both"):
+        c["k_lens"] = torch.randint(0, Lk + 1, (B,), generator=g, dtype=torch.int32)
+        c["k_lens"][0] = Lk
+    return c, do
+
+
+def to(c, dev):
+    return {n: None if t is None else t.to(dev) for n, t in c.items()}
+
+
+def run_cross(c, do, gpu, scale=None, names=("q", "k", "v", "bias")):
+    d = to(c, gpu)
+    leaves = [d[n].requires_grad_() for n in names if d[n] is not None]
+    o = ops.cross_attention(**d, scale=scale)
+    return o, dict(zip(["d" + n for n in names if d[n] is not None], torch.autograd.grad(o, leaves, do.to(gpu))))
+
+
+def check_cross(c, do, gpu, scale=None):
+    dtype = c["q"].dtype
+    r = ref.cross_attention(**c, scale=scale, do=do)
+    slack = ref.cross_attention_slack(r, dtype, c["bias"])
+    plain = ops.cross_attention(**to(c, gpu), scale=scale)
+    o, grads = run_cross(c, do, gpu, scale)
+    assert torch.equal(plain, o.detach())
+    check(o.detach(), r["o"], slack["o"])
+    for n, got in grads.items():
+        want, s = r[n], slack[n]
+        if n == "dbias":
+            for d in (0, 1):
+                if c["bias"].shape[d] == 1 and want.shape[d] != 1:
+                    m = want.shape[d]
+                    s = s.sum(d, keepdim=True) + m * U32 * want.abs().sum(d, keepdim=True)
+                    want = want.sum(d, keepdim=True)
+        check(got, want, s)
+    return o, grads
+
+
+CROSS = [  # B, Lq, Lk, H, Hk, D
+    (1, 1, 1, 1, 1, 8), (2, 1, 33, 4, 4, 24), (3, 1, 300, 8, 2, 64), (2, 32, 128, 4, 4, 32), (1, 33, 127, 4, 4, 32),
+    (2, 5, 129, 6, 2, 128), (1, 130, 64, 2, 2, 48), (2, 70, 200, 4, 1, 40), (1, 257, 65, 2, 1, 96), (1, 3, 1030, 2, 2, 16),
+    (1, 129, 515, 1, 1, 128), (1, 40, 700, 3, 3, 56)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias,hide", [(None, None), ("full", "mask"), ("b1 own", "lens"), ("h1", "both")])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D", CROSS)
+def test_cross_attention(gpu, B, Lq, Lk, H, Hk, D, bias, hide, dtype):
+    c, do = inputs(Lq + Lk + D, dtype, B, Lq, Lk, H, Hk, D, bias, hide)
+    check_cross(c, do, gpu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.7])
+def test_cross_attention_scales(gpu, dtype, scale):
+    c, do = inputs(3, dtype, 2, 40, 90, 2, 2, 32, "full", "mask")
+    o, grads = check_cross(c, do, gpu, scale)
+    if scale == 0.0:
+        assert not grads["dq"].any() and not grads["dk"].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_cross_attention_peaked(gpu, dtype, Lq):
+    """Logits of some hundreds: nearly all weight on one key, and most probabilities 0."""
+    c, do = inputs(4, dtype, 2, Lq, 150, 2, 2, 64, "full", "lens", scale=40.0)
+    c["bias"] *= 30
+    check_cross(c, do, gpu)
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -12, 2.0 ** 6])
+def test_cross_attention_fp16_gradients_of_any_size(gpu, factor):
+    """Small and large output gradients: dS lies outside fp16's range, its sums do not."""
+    c, do = inputs(5, torch.float16, 1, 70, 600, 4, 2, 32)
+    check_cross(c, (do.float() * factor).half(), gpu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Lq,Lk,D", [(1, 130, 64), (50, 130, 32), (150, 70, 128)])
+@pytest.mark.parametrize("bias", [None, "full"])
+def test_cross_attention_rows_that_see_nothing(gpu, dtype, Lq, Lk, D, bias):
+    """Batch element 0: every key masked; 1: length 0; 2: all but one key hidden; with a bias, element 3's
+    queries hide all keys from themselves every third row."""
+    c, do = inputs(6, dtype, 4, Lq, Lk, 2, 2, D, bias, "both")
+    c["mask"][:], c["k_lens"][:] = True, Lk
+    c["mask"][0], c["k_lens"][1], c["mask"][2] = False, 0, False
+    c["mask"][2, Lk // 2] = True
+    if bias:
+        c["bias"][3, :, ::3] = -torch.inf
+        c["bias"][3, :, 1::3, ::2] = -torch.inf
+    o, grads = check_cross(c, do, gpu)
+    for t in (o, grads["dq"], grads["dk"], grads["dv"]):
+        assert not t[:2].any()
+    assert torch.equal(o[2].cpu(), c["v"][2, Lk // 2].expand(Lq, 2, D))
+    if bias:
+        assert not grads["dbias"][:2].any() and not o[3, ::3].any() and not grads["dq"][3, ::3].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf"), None])
+@pytest.mark.parametrize("Lq", [1, 60])
+def test_cross_attention_ignores_what_is_hidden(gpu, dtype, junk, Lq):
+    """NaN, infinities and the lowest value in hidden keys, values and biases change no bit."""
+    c, do = inputs(7, dtype, 2, Lq, 140, 4, 2, 32, "full", "both")
+    c["k_lens"][1] = 77
+    hidden = ~ref.cross_attention(**c)["seen"]
+    clean, grads = run_cross(c, do, gpu)
+    bad = torch.finfo(dtype).min if junk is None else junk
+    for n in "kv":
+        c[n][hidden] = bad
+    c["bias"] = torch.where(hidden[:, None, None], torch.full((), torch.finfo(torch.float32).min if junk is None else junk), c["bias"])
+    o, dirty = run_cross(c, do, gpu)
+    assert torch.equal(o, clean) and all(torch.equal(grads[n], dirty[n]) for n in grads)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_attention_lowest_value_as_a_mask(gpu, dtype):
+    """A bias of fp32's lowest value hides a key as long as another is there; a row of nothing else sees all its
+    keys alike, as fp32 softmax does (the logits vanish next to it)."""
+    c, do = inputs(8, dtype, 1, 40, 100, 2, 2, 32, "full")
+    low = torch.finfo(torch.float32).min
+    c["bias"][:, :, :20, 50:] = low
+    c["bias"][:, :, 20:] = low
+    o, grads = run_cross(c, do, gpu)
+    first = {**c, "q": c["q"][:, :20], "k": c["k"][:, :50], "v": c["v"][:, :50], "bias": c["bias"][:, :, :20, :50]}
+    r = ref.cross_attention(**first)
+    check(o[:, :20].detach(), r["o"], ref.cross_attention_slack(r, dtype, first["bias"])["o"])
+    rest = {**c, "q": c["q"][:, 20:], "bias": None}
+    r = ref.cross_attention(**rest, scale=0.0, do=do[:, 20:])
+    slack = ref.cross_attention_slack(r, dtype)
+    check(o[:, 20:].detach(), r["o"], slack["o"])
+    check(grads["dbias"][:, :, 20:], r["dbias"], slack["dbias"])   # P is 1 / 100 there, not 1
+    assert torch.isfinite(grads["dq"]).all() and grads["dv"].abs().max() < 100
+
+
+def test_cross_attention_visible_nan_spreads(gpu):
+    c, _ = inputs(9, torch.float32, 2, 5, 200, 2, 2, 32)
+    c["q"][0, 1, 0, 3] = float("nan")
+    c["k"][1, 150, 1, 3] = float("nan")
+    bad = ops.cross_attention(**to(c, gpu)).isnan().all(3).cpu()
+    want = torch.zeros((2, 5, 2), dtype=torch.bool)
+    want[0, 1, 0] = True
+    want[1, :, 1] = True
+    assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_attention_strides(gpu, dtype):
+    """Views of a fused projection, permuted heads, shared batches, biases in [B, Lq, Lk, H], offset bases."""
+    c, do = inputs(10, dtype, 2, 37, 100, 4, 4, 32, "full", "mask")
+    d = to(c, gpu)
+    do = do.to(gpu)
+
+    def run(x):
+        leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v", "bias")]
+        o = ops.cross_attention(*leaves[:3], bias=leaves[3], mask=x["mask"])
+        return [o, *torch.autograd.grad(o, leaves, do)]
+    want = run(d)
+    kv = torch.cat([d["k"], d["v"]], 3)                       # [B, Lk, H, 2 D]
+    views = [{**d, "k": kv[..., :32], "v": kv[..., 32:]},
+             {**d, "q": d["q"].transpose(1, 2).contiguous().transpose(1, 2)},
+             {**d, "k": d["k"].permute(1, 2, 0, 3).contiguous().permute(2, 0, 1, 3)},
+             {**d, "v": d["v"].transpose(2, 3).contiguous().transpose(2, 3)},
+             {**d, "q": torch.cat([d["q"].flatten()[:1], d["q"].flatten()])[1:].view(d["q"].shape)},
+             {**d, "bias": d["bias"].permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)},
+             {**d, "bias": torch.cat([d["bias"].flatten()[:1], d["bias"].flatten()])[1:].view(d["bias"].shape)},
+             {**d, "mask": d["mask"].t().contiguous().t()}, {**d, "mask": d["mask"].float() * 3}]
+    for x in views:
+        assert all(torch.equal(a, b) for a, b in zip(run(x), want))
+    one = {**d, "k": d["k"][:1].expand(2, -1, -1, -1), "v": d["v"][:1].expand(2, -1, -1, -1), "mask": d["mask"][:1]}
+    two = {**d, "k": d["k"][:1].repeat(2, 1, 1, 1), "v": d["v"][:1].repeat(2, 1, 1, 1), "mask": d["mask"][:1].repeat(2, 1)}
+    assert all(torch.equal(a, b) for a, b in zip(run(one), run(two)))
+    grad = do.transpose(1, 2).contiguous().transpose(1, 2)
+    q = d["q"].detach().requires_grad_()
+    o = ops.cross_attention(q, d["k"], d["v"], d["bias"], d["mask"])
+    assert torch.equal(*(torch.autograd.grad(o, q, g, retain_graph=True)[0] for g in (grad, do)))
+
+
+@pytest.mark.parametrize("names", [("q",), ("k",), ("v",), ("bias",), ("k", "bias"), ("q", "v")])
+def test_cross_attention_partial_gradients(gpu, names):
+    c, do = inputs(11, torch.bfloat16, 2, 37, 100, 4, 2, 32, "b1", "mask")
+    # (delta is formed in another way where the bias has a gradient)
+    _, every = run_cross(c, do, gpu, names=("q", "k", "v", "bias")[:4 if "bias" in names else 3])
+    _, some = run_cross(c, do, gpu, names=names)
+    assert set(some) == {"d" + n for n in names} and all(torch.equal(some[n], every[n]) for n in some)
+
+
+def test_cross_attention_empties(gpu):
+    for B, Lq, Lk, H in ((2, 3, 0, 2), (2, 0, 5, 2), (0, 3, 5, 2), (1, 40, 0, 2)):
+        q, k = torch.ones((B, Lq, H, 16), device=gpu), torch.ones((B, Lk, H, 16), device=gpu)
+        bias = torch.ones((B, H, Lq, Lk), device=gpu)
+        leaves = [t.requires_grad_() for t in (q, k, k.detach().clone(), bias)]
+        o = ops.cross_attention(*leaves[:3], bias=bias)
+        assert o.shape == q.shape and not o.any()
+        for g, t in zip(torch.autograd.grad(o, leaves, torch.ones_like(o)), leaves):
+            assert g.shape == t.shape and not g.any()
+
+
+def test_cross_attention_lengths_are_clamped(gpu):
+    c, _ = inputs(12, torch.float16, 4, 5, 60, 2, 2, 32)
+    d = to(c, gpu)
+    lens = torch.tensor([-7, 0, 60, 10 ** 6], device=gpu)
+    got = ops.cross_attention(d["q"], d["k"], d["v"], k_lens=lens)
+    assert not got[:2].any() and torch.equal(got[2:], ops.cross_attention(d["q"], d["k"], d["v"])[2:])
+    assert torch.equal(got, ops.cross_attention(d["q"], d["k"], d["v"], k_lens=lens.int()))
+    far = torch.tensor([2 ** 40, -2 ** 40, 2 ** 32 + 1, 3], device=gpu)
+    got = ops.cross_attention(d["q"], d["k"], d["v"], k_lens=far)
+    assert not got[1].any() and torch.equal(got[::2], ops.cross_attention(d["q"], d["k"], d["v"])[::2])
+
+
+def test_cross_attention_offsets_past_32_bits(gpu):
+    """Batch elements and heads 2^31 elements apart."""
+    buf = torch.empty(2 ** 32 + 2 ** 21, dtype=torch.float16, device=gpu)
+    k = buf.as_strided((2, 70, 2, 32), (2 ** 31, 64, 32, 1))
+    v = buf.as_strided((2, 70, 2, 32), (2 ** 20, 64, 2 ** 32, 1), 8192)
+    k.copy_(torch.randn(k.shape, device=gpu)), v.copy_(torch.randn(v.shape, device=gpu))
+    for Lq in (1, 50):
+        q, do = torch.randn((2, Lq, 4, 32), device=gpu).half().requires_grad_(), torch.randn((2, Lq, 4, 32), device=gpu).half()
+        o, p = ops.cross_attention(q, k, v), ops.cross_attention(q, k.contiguous(), v.contiguous())
+        assert torch.equal(o, p) and torch.equal(torch.autograd.grad(o, q, do)[0], torch.autograd.grad(p, q, do)[0])
+
+
+def test_cross_attention_gradients_by_differences(gpu):
+    """fp32, a few directions: (f(x + e) - f(x - e)) / 2 with e of size 2^-7 of x; the third derivative's part is of
+    relative order e^2 / 6 (a factor of 16 is allowed for its size), fp32 roundings of f are divided by e."""
+    c, do = inputs(13, torch.float32, 1, 6, 20, 2, 1, 16, "full")
+    _, grads = run_cross(c, do, gpu)
+    g = torch.Generator().manual_seed(14)
+    for n in ("q", "k", "v", "bias"):
+        e = normal(g, *c[n].shape) * 2.0 ** -7
+        f = [(ops.cross_attention(**to({**c, n: c[n] + s * e}, gpu)).double().cpu() * do.double()).sum() for s in (1, -1)]
+        want = (f[0] - f[1]) / 2
+        got = (grads["d" + n].double().cpu() * e.double()).sum()
+        size = (grads["d" + n].double().cpu().abs() * e.double().abs()).sum()
+        r = ref.cross_attention(**c, do=do)
+        slack = ref.cross_attention_slack(r, torch.float32, c["bias"])["o"]
+        assert abs(want - got) <= 16 / 6 * 2.0 ** -14 * size + (slack * do.double().abs()).sum()
+
+
+def test_cross_attention_same_bits_each_time(gpu):
+    for dtype in DTYPES:
+        c, do = inputs(15, dtype, 2, 300, 500, 4, 2, 64, "h1", "both")
+        first = run_cross(c, do, gpu)
+        again = run_cross(c, do, gpu)
+        assert torch.equal(first[0], again[0]) and all(torch.equal(first[1][n], again[1][n]) for n in first[1])
+
+
+# ------------------------------------------------------------------------------ a run of them together
+class Block:
+    """Token rows broadcast to their atoms, atoms attending over another track, a dropped-out residual update and the
+    sum of atoms by token."""
+
+    def __init__(self, gpu, dtype, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        self.tokens, self.atoms, self.H, self.D = 40, 150, 4, 16
+        c = self.H * self.D
+        self.w = normal(g, self.tokens, c, dtype=dtype).to(gpu)
+        self.kv = normal(g, 1, 70, 2, self.H, self.D, dtype=dtype).to(gpu)
+        self.bias = normal(g, self.H, self.atoms, 70).to(gpu)
+        self.owner = tokens(g, "sorted", self.atoms, self.tokens).to(gpu)
+        self.lens = torch.tensor([61], device=gpu, dtype=torch.int32)
+        self.do = normal(g, self.tokens, c, dtype=dtype).to(gpu)
+
+    def run(self, seed):
+        leaves = [t.detach().requires_grad_() for t in (self.w, self.kv, self.bias)]
+        w, kv, bias = leaves
+        x = ops.embedding(self.owner, w, 0.5)
+        q = x.view(1, self.atoms, self.H, self.D)
+        a = ops.cross_attention(q, kv[:, :, 0], kv[:, :, 1], bias=bias, k_lens=self.lens)
+        y = ops.dropout_add(a.reshape(x.shape), x, 0.25, seed, 3)
+        out = ops.embedding_grad(y, self.owner, self.tokens)   # sums by token; its own gradient is a lookup
+        return [y.detach(), out.detach(), *torch.autograd.grad(out, leaves, self.do)]
+
+    def plain(self, seed):
+        leaves = [t.detach().cpu().double().requires_grad_() for t in (self.w, self.kv, self.bias)]
+        w, kv, bias = leaves
+        owner = self.owner.cpu()
+        inside = (owner >= 0)[:, None]
+        x = torch.where(inside, w[owner.clamp_min(0)] * 0.5, torch.zeros((), dtype=torch.float64))
+        q = x.view(1, self.atoms, self.H, self.D).transpose(1, 2)
+        k, v = kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+        logits = q @ k.transpose(2, 3) / self.D ** 0.5 + bias
+        logits = logits.masked_fill(torch.arange(70) >= self.lens.cpu(), -torch.inf)
+        a = (torch.softmax(logits, 3) @ v).transpose(1, 2).reshape(x.shape)
+        y = x + a * ref.dropout_keep(x.shape, 0.25, seed, 3).double() / 0.75
+        out = torch.zeros((self.tokens, x.shape[1]), dtype=torch.float64).index_add(0, owner.clamp_min(0), y * inside)
+        return [y.detach(), out.detach(), *torch.autograd.grad(out, leaves, self.do.cpu().double())]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_block(gpu, dtype):
+    """Every operator rounds its result to the type once and the products' operands once: eight roundings follow
+    each other on the longest way (lookup, o, residual, dS, dq, the residual's gradient, their sum, dw); each is
+    at most half a step of a value, and within a gradient's row values differ by less than its largest."""
+    b = Block(gpu, dtype)
+    for got, want in zip(b.run(77), b.plain(77)):
+        tol = (8 * torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 512 * U32) * 4 * want.abs().max()
+        assert (got.double().cpu() - want).abs().max() <= tol
+
+
+def test_block_in_a_graph(gpu):
+    """Forward and backward captured together (torch.autograd.grad: no accumulation), replayed with new inputs, other
+    eager work and synchronizations between."""
+    b = Block(gpu, torch.bfloat16)
+    seed = torch.tensor([5], device=gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b.run(seed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = b.run(seed)
+    for s in range(4):
+        new = Block(gpu, torch.bfloat16, seed=s)
+        for n in ("w", "kv", "bias", "owner", "do"):
+            getattr(b, n).copy_(getattr(new, n))
+        b.lens.fill_(70 - 20 * s)
+        seed.fill_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, b.run(s)))
+
+
+def test_cross_attention_launchers_in_two_graphs(gpu):
+    """Two captured steps with workspaces of their own, replayed on two streams at once."""
+    graphs = []
+    for seed in (1, 2):
+        c, do = inputs(seed, torch.float16, 2, 20, 900, 4, 2, 64, "b1", "both")
+        d, do = to(c, gpu), do.to(gpu)
+        o, o32 = torch.empty_like(d["q"]), torch.empty(d["q"].shape, device=gpu)
+        stats = torch.empty((2, 2, 4, 20), device=gpu)
+        dq, dk, dv, db = (torch.empty_like(d[n]) for n in ("q", "k", "v", "bias"))
+        ws = ops.workspace(ops.cross_attention_workspace_bytes(d["q"], d["k"]), gpu)
+        wb = ops.workspace(ops.cross_attention_bwd_workspace_bytes(d["q"], d["k"], d["bias"]), gpu)
+        more = dict(bias=d["bias"], mask=d["mask"], k_lens=d["k_lens"])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.launch_cross_attention(d["q"], d["k"], d["v"], o, o32=o32, stats=stats, ws=ws, **more)
+            ops.launch_cross_attention_bwd(do, d["q"], d["k"], d["v"], o, o32, stats, dq, dk, dv, wb, dbias=db, **more)
+        graphs.append((graph, c, do.cpu(), (o, dq, dk, dv, db), (ws, wb), (d, do, o32, stats)))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for _, _, _, outs, ws, _ in graphs:
+            for t in (*outs, *ws):
+                t.fill_(float("nan") if t.is_floating_point() else 255)
+        torch.cuda.synchronize()
+        for (graph, *_), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, c, do, outs, _, _ in graphs:
+            o, grads = run_cross(c, do, gpu)
+            assert all(torch.equal(x, y) for x, y in zip(outs, (o, grads["dq"], grads["dk"], grads["dv"], grads["dbias"])))

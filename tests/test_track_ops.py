@@ -148,3 +148,89 @@ def test_abi_refuses_without_launching():
         assert re.search(say, _err()), (change, _err())
     assert lib.pf_dropout_add_fwd(None) == -1 and "null args" in _err()
     assert lib.pf_dropout_add_fwd(ctypes.byref(_lib.DropoutArgs(**{**ok, "C": 0}))) == 0
+
+
+# ------------------------------------------------------------------------------ cross attention
+def test_cross_attention_oracle_against_autograd():
+    g = torch.Generator().manual_seed(0)
+    shapes = dict(q=(2, 5, 4, 8), k=(2, 7, 2, 8), v=(2, 7, 2, 8), bias=(2, 4, 5, 7))
+    t = {n: torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True) for n, s in shapes.items()}
+    mask, do = torch.rand((2, 7), generator=g) < 0.7, torch.randn((2, 5, 4, 8), generator=g, dtype=torch.float64)
+    k, v = (t[n].transpose(1, 2).repeat_interleave(2, 1) for n in "kv")
+    o = torch.nn.functional.scaled_dot_product_attention(t["q"].transpose(1, 2), k, v,
+                                                         t["bias"].masked_fill(~mask[:, None, None], -torch.inf)).transpose(1, 2)
+    want = [o, *torch.autograd.grad(o, list(t.values()), do)]
+    r = ref.cross_attention(**t, mask=mask, do=do)
+    for n, w in zip(("o", "dq", "dk", "dv", "dbias"), want):
+        assert (r[n] - w).abs().max() < 1e-13
+
+
+def _cross(dtype=torch.float32, B=2, Lq=5, Lk=7, H=4, Hk=2, D=16):
+    return torch.zeros((B, Lq, H, D), dtype=dtype), torch.zeros((B, Lk, Hk, D), dtype=dtype), torch.zeros((B, Lk, Hk, D), dtype=dtype)
+
+
+def test_cross_attention_refuses(lib):
+    q, k, v = _cross()
+    bias = torch.zeros((2, 4, 5, 7))
+    for args, kw, say in (((q[0], k, v), {}, "expects q"), ((q, k[0], v), {}, "expects q"), ((q, k, v[:, :6]), {}, "do not fit"),
+                          ((q, k[:1], v[:1]), {}, "do not fit"), ((q, k[..., :8], v[..., :8]), {}, "do not fit"),
+                          ((q[:, :, :3], k, v), {}, "do not fit"), ((q, k[:, :, :0], v[:, :, :0]), {}, "do not fit"),
+                          ((q, k.half(), v), {}, "differ in type"), ((q.double(), k.double(), v.double()), {}, "element type"),
+                          ((q[..., :12], k[..., :12], v[..., :12]), {}, "multiple of 8"), (_cross(D=136), {}, "multiple of 8"),
+                          ((q, k, v), {"scale": float("nan")}, "finite"), ((q, k, v), {"scale": float("inf")}, "finite"),
+                          ((q, k, v), {"bias": bias[0, 0, 0]}, "expects bias"), ((q, k, v), {"bias": bias[..., :6]}, "does not fit"),
+                          ((q, k, v), {"bias": bias[:, :, :1]}, "does not fit"), ((q, k, v), {"bias": bias[:, :3]}, "does not fit"),
+                          ((q, k, v), {"bias": bias.half()}, "bias is"), ((q, k, v), {"k_lens": torch.zeros(3, dtype=torch.int32)}, "k_lens"),
+                          ((q, k, v), {"k_lens": torch.zeros(2)}, "k_lens")):
+        with pytest.raises(ValueError, match=say):
+            ops.cross_attention(*args, **kw)
+    for mask in (torch.ones((2, 6)), torch.ones((3, 7)), torch.ones((2, 1, 7))):
+        with pytest.raises(RuntimeError):
+            ops.cross_attention(q, k, v, mask=mask)
+    assert not lib.calls
+
+
+def test_cross_attention_reads_views_in_place(lib):
+    kv = torch.zeros((2, 7, 2, 32))
+    q, bias = torch.zeros((2, 4, 5, 16)).transpose(1, 2), torch.zeros((4, 5, 7))
+    ops.cross_attention(q, kv[..., :16], kv[..., 16:], bias=bias, mask=torch.ones(7))
+    (name, (a,)), = [c for c in lib.calls]
+    a = a._obj
+    assert name == "pf_cross_attn_fwd" and (a.B, a.Lq, a.Lk, a.H, a.Hk, a.D) == (2, 5, 7, 4, 2, 16)
+    assert a.q == q.data_ptr() and (a.q_b, a.q_l, a.q_h) == (320, 16, 80)
+    assert a.v == kv.data_ptr() + 64 and (a.v_b, a.v_l, a.v_h) == (448, 64, 32)
+    assert a.bias == bias.data_ptr() and (a.bias_b, a.bias_h, a.bias_q, a.bias_k) == (0, 35, 7, 1) and a.mask_b == 0
+    assert a.o32 is None and a.stats is None
+    lib.calls.clear()
+    ops.cross_attention(q, kv[..., 1:17], kv[..., :16])   # not in 16-byte pieces: a copy
+    a = lib.calls[0][1][0]._obj
+    assert a.k != kv.data_ptr() + 4 and (a.k_b, a.k_l, a.k_h) == (224, 32, 16)
+
+
+def test_cross_attention_abi_refuses_without_launching():
+    lib, d = _lib.load(), 4096
+    ok = dict(B=2, Lq=5, Lk=7, H=4, Hk=2, D=16, scale=0.25, q=d, q_b=320, q_l=64, q_h=16, k=d, k_b=224, k_l=32, k_h=16, v=d,
+              v_b=224, v_l=32, v_h=16, o=d)
+    for change, say in ((dict(dtype=5), "dtype"), (dict(D=20), "D must"), (dict(D=136), "D must"), (dict(H=3), "bad shape"),
+                        (dict(Hk=0), "bad shape"), (dict(B=-1), "bad shape"), (dict(scale=float("nan")), "finite"), (dict(q=None), "null"),
+                        (dict(k=None), "null"), (dict(o=None), "null"), (dict(q=d + 4), "aligned"), (dict(k_l=34), "strides"),
+                        (dict(o=d + 8), "aligned"), (dict(bias=d, bias_dtype=1), "bias"), (dict(Lk=1 << 30), "too long"),
+                        (dict(B=1 << 20, Lq=1 << 20), "too large")):
+        a = _lib.CrossAttnArgs(**{**ok, **change})
+        assert lib.pf_cross_attn_fwd(ctypes.byref(a)) == -1 and say in _err(), (change, _err())
+    assert lib.pf_cross_attn_fwd(None) == -1 and "null args" in _err()
+    assert lib.pf_cross_attn_fwd(ctypes.byref(_lib.CrossAttnArgs(**{**ok, "Lq": 0}))) == 0
+    long = _lib.CrossAttnArgs(**{**ok, "Lk": 100000})
+    need = lib.pf_cross_attn_workspace_size(ctypes.byref(long))
+    assert need > 0 and lib.pf_cross_attn_fwd(ctypes.byref(long)) == -1 and "workspace too small" in _err()
+    long.workspace, long.workspace_bytes = d + 4, need
+    assert lib.pf_cross_attn_fwd(ctypes.byref(long)) == -1 and "aligned" in _err()
+    back = {**ok, "stats": d, "dout": d, "dq": d, "dk": d, "dv": d, "workspace": d, "workspace_bytes": 1 << 30}
+    for change, say in ((dict(stats=None), "statistics"), (dict(dout=None), "dout"), (dict(dtype=1), "unrounded"), (dict(dv=None), "come together"),
+                        (dict(dbias=d, dbias_B=2, dbias_H=4), "does not belong"), (dict(dbias_B=2, dbias_H=4), "do not agree"),
+                        (dict(bias=d, dbias=d, dbias_B=1, dbias_H=4, dq=None), "comes with dq"),
+                        (dict(bias=d, dbias=d, dbias_B=3, dbias_H=4), "does not belong"), (dict(workspace_bytes=16), "workspace too small"),
+                        (dict(dq=d + 4), "aligned"), (dict(Lq=0), "no queries")):
+        a = _lib.CrossAttnArgs(**{**back, **change})
+        assert lib.pf_cross_attn_bwd(ctypes.byref(a)) == -1 and say in _err(), (change, _err())
+    assert lib.pf_cross_attn_bwd(None) == -1 and "null args" in _err()

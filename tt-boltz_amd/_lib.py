@@ -132,6 +132,22 @@ class DropoutArgs(ctypes.Structure):
     ]
 
 
+class CrossAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int), ("Lq", c_int), ("Lk", c_int), ("H", c_int), ("Hk", c_int), ("D", c_int),
+        ("dtype", c_int), ("bias_dtype", c_int), ("scale", c_float),
+        ("q", c_void_p), ("q_b", c_long), ("q_l", c_long), ("q_h", c_long),
+        ("k", c_void_p), ("k_b", c_long), ("k_l", c_long), ("k_h", c_long),
+        ("v", c_void_p), ("v_b", c_long), ("v_l", c_long), ("v_h", c_long),
+        ("bias", c_void_p), ("bias_b", c_long), ("bias_h", c_long), ("bias_q", c_long), ("bias_k", c_long),
+        ("mask", c_void_p), ("mask_b", c_long), ("k_lens", c_void_p),
+        ("o", c_void_p), ("o32", c_void_p), ("stats", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("stream", c_void_p),
+        ("dout", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dbias", c_void_p),
+        ("dbias_B", c_int), ("dbias_H", c_int),
+    ]
+
+
 #: name -> (restype, argtypes); every symbol include/pairformer_hip.h declares.
 SIGNATURES = {
     "pf_abi_version": (c_int, []),
@@ -189,6 +205,10 @@ SIGNATURES = {
     "pf_embedding_grad_workspace_size": (c_size_t, [c_long, c_long, c_long]),
     "pf_embedding_grad": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_long, c_long, c_long, c_int, c_float, c_void_p,
                                   c_size_t, c_void_p]),
+    "pf_cross_attn_workspace_size": (c_size_t, [ctypes.POINTER(CrossAttnArgs)]),
+    "pf_cross_attn_fwd": (c_int, [ctypes.POINTER(CrossAttnArgs)]),
+    "pf_cross_attn_bwd_workspace_size": (c_size_t, [ctypes.POINTER(CrossAttnArgs)]),
+    "pf_cross_attn_bwd": (c_int, [ctypes.POINTER(CrossAttnArgs)]),
     "pf_dropout_add_fwd": (c_int, [ctypes.POINTER(DropoutArgs)]),
     "pf_attend_timing": (c_int, [c_int]),
     "pf_attend_timing_read": (c_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_int)]),

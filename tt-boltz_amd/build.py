@@ -20,7 +20,7 @@ OBJDIR = os.path.join(HERE, "_build")
 SOURCES = ["api.cpp", "trimul.hip", "triatt.hip", "transition.hip", "single.hip", "fast8.hip", "msa.hip", "diffusion.hip",
            "pad.hip", "measure.hip"]
 #: sources that work in the caller's element type: compiled once, linked into every library
-COMMON_SOURCES = ["embed.hip", "dropout.hip"]
+COMMON_SOURCES = ["cross_fp32.hip", "cross_fp16.hip", "cross_bf16.hip", "cross_attn.hip", "embed.hip", "dropout.hip"]
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

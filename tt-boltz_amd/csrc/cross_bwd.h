@@ -1,0 +1,474 @@
+// Backward pass of cross attention, included once per element type after cross_kernels.h (see there).
+//
+// Two kernels, neither with atomics, so gradients are the same bits each time: xa_dq_kernel (a
+// workgroup has queries, walks over keys; also writes the logits' gradient where a bias wants it) and
+// xa_dkv_kernel (a workgroup has 128 keys, walks over the rows of all heads that share them).
+//
+// fp16: dS and P are products' operands and far smaller than 1, where fp16 has few bits left (below
+// 2^-14) or none (2^-25).  P is taken 2^15 times larger, and dS by the power of two that brings its
+// bound max|do_i| max|v_j| 2 to 2^14 or less; both factors are divided out of the fp32 sums.
+#pragma once
+#include "cross_kernels.h"
+
+namespace {
+
+template <typename T>
+constexpr bool SCALED = __is_same(T, half_t);
+
+// power of two that brings 2 |do| |v| to (2^13, 2^14] (1 where the bound is 0 or not finite)
+PF_DEV float ds_scale(const XaParams& p, int b, int hk) {
+  const uint32_t* a = p.amax + 2 * ((long)b * p.Hk + hk);
+  const float bound = 2.f * __fsqrt_rn(__uint_as_float(a[0])) * __fsqrt_rn(__uint_as_float(a[1]));
+  if (!(bound > 0.f) || !(bound < 3.0e38f)) return 1.f;
+  int e;
+  (void)frexpf(bound, &e);
+  return ldexpf(1.f, max(-100, min(14 - e, 100)));
+}
+
+// ------------------------------------------------------------------------------ delta
+// delta_i = do_i . o_i in fp32 from the unrounded o (delta null: not wanted), 8 lanes a row.  fp16: also the largest |do_i|^2
+// and |v_j|^2 of a key head (maxima of non-negative floats as whole numbers: any order gives the same).
+template <typename T>
+__global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __restrict__ delta, uint32_t* amax) {
+  const long rows = (long)p.B * p.Lq * p.H, keys = SCALED<T> ? (long)p.B * p.Lk * p.Hk : 0;
+  const int sub = threadIdx.x & 7;
+  const float* o32 = p.o32 ? p.o32 : (const float*)p.o;
+  const long row = ((long)blockIdx.x * 256 + threadIdx.x) >> 3;
+  float dot = 0.f, sq = 0.f;
+  if (row < rows) {
+    for (int d = 4 * sub; d < p.D; d += 32)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float g = (float)((const T*)p.dout)[row * p.D + d + e];
+        if (delta) dot += g * o32[row * p.D + d + e];
+        sq += g * g;
+      }
+  } else if (row < rows + keys) {
+    const long j = row - rows, bl = j / p.Hk, b = bl / p.Lk;
+    const int hk = (int)(j - bl * p.Hk), key = (int)(bl - b * p.Lk);
+    const bool seen = key < length_of(p, (int)b) && (!p.mask || p.mask[b * p.mb + key]);
+    const T* v = (const T*)p.v + b * p.vb + key * p.vl + hk * p.vh;
+    if (seen)
+      for (int d = 4 * sub; d < p.D; d += 32)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float g = (float)v[d + e];
+          sq += g * g;
+        }
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    dot += __shfl_xor(dot, o);
+    sq += __shfl_xor(sq, o);
+  }
+  if (sub != 0) return;
+  if (row < rows) {
+    const long bl = row / p.H;
+    const int head = (int)(row - bl * p.H);
+    const long b = bl / p.Lq, i = bl - b * p.Lq;
+    if (delta) delta[(b * p.H + head) * p.Lq + i] = dot;
+    if constexpr (SCALED<T>) atomicMax(amax + 2 * (b * p.Hk + head / p.G), __float_as_uint(sq));
+  } else if (row < rows + keys) {
+    const long j = row - rows, bl = j / p.Hk;
+    atomicMax(amax + 2 * (bl / p.Lk * p.Hk + (j - bl * p.Hk)) + 1, __float_as_uint(sq));
+  }
+}
+
+// ------------------------------------------------------------------------------ dq, dS
+// DELTA: delta_i = sum_j P_ij (do_i . v_j) instead, of the split's keys, from the fp32 P and dP that dS will
+// be made of.  A bias's gradient is dS itself, in fp32 as a rule, and do . o is not good enough for it:
+// 16-bit types round P in o's product (2^-9 or 2^-12 of delta, against 2^-22 here).
+template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
+__global__ __launch_bounds__(256) void xa_dq_kernel(XaParams p) {
+  using M = Mma<T>;
+  constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
+  constexpr int KS = M::row_stride(DP);
+  extern __shared__ __align__(16) char smem[];
+  T* const ks = reinterpret_cast<T*>(smem);
+  T* const vs = ks + KT * KS;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+  constexpr int ROWS = FEW ? 32 : 128;
+  const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
+  const int b = blk.b, hk = blk.hk;
+  const int r = blk.rt * ROWS + (FEW ? 0 : 32 * wid) + n;
+  const bool row_ok = r < p.rows;
+  const int i = row_ok ? r / p.G : 0, head = hk * p.G + (row_ok ? r - i * p.G : 0);
+  const int sub0 = FEW ? 32 * wid : 0;
+  const long row_at = ((long)b * p.Lq + i) * p.H + head;
+  Frag<T, DP> q, g;
+  q.load((const T*)p.q + b * p.qb + i * p.ql + head * p.qh, p.D, h, row_ok, p.neg);
+  g.load((const T*)p.dout + row_at * p.D, p.D, h, row_ok);
+  const long stat = ((long)b * p.H + head) * p.Lq + i;
+  const float m = row_ok ? p.st_m[stat] : 0.f, ll = row_ok ? p.st_l[stat] : INFINITY;
+  const float delta = !DELTA && row_ok ? p.delta[stat] : 0.f;
+  const float sf = SCALED<T> && !DELTA ? ds_scale(p, b, hk) : 1.f;
+  float sum = 0.f;   // DELTA: this lane's half of the keys
+  const char* bias = nullptr;
+  bool bias_vec = false;
+  if constexpr (BIAS) {
+    const long at = b * p.bb + head * p.bh + i * p.bq;
+    bias = (const char*)p.bias + at * (p.bias_f32 ? 4 : (long)sizeof(T));
+    bias_vec = p.bk == 1 && ((p.bb | p.bh | p.bq) & 3) == 0 && ((uintptr_t)p.bias & 15) == 0;
+  }
+  float* const ds = !DELTA && p.ds && row_ok ? p.ds + stat * p.Lk : nullptr;
+  const bool ds_vec = (p.Lk & 3) == 0;
+  const int len = length_of(p, b);
+  // the logits' gradient has zeros at hidden keys, so its writer goes on to the end
+  const int t0 = blk.z * p.per, t1 = min(t0 + p.per, ((!DELTA && p.ds ? p.Lk : len) + KT - 1) / KT);
+  const uint8_t* mask = p.mask ? p.mask + b * p.mb : nullptr;
+  const T* const kb = (const T*)p.k + b * p.kb + hk * p.kh;
+  const T* const vb = (const T*)p.v + b * p.vb + hk * p.vh;
+
+  Stage<T, DP, KT> sk, sv;
+  auto load_tile = [&](int t) __attribute__((always_inline)) {
+    auto seen = [&](int row) __attribute__((always_inline)) {
+      const int key = t * KT + row;
+      return key < len && (!mask || mask[key]);
+    };
+    sk.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? kb + (long)(t * KT + row) * p.kl : nullptr; });
+    sv.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? vb + (long)(t * KT + row) * p.vl : nullptr; });
+  };
+
+  const float c = BIAS ? p.scale : p.scale * LOG2E;
+  f32x16 dq[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
+
+  if (t0 < t1) load_tile(t0);
+  for (int t = t0; t < t1; ++t) {
+    sk.store(ks, KS);
+    sv.store(vs, KS);
+    __syncthreads();
+    if (t + 1 < t1) load_tile(t + 1);
+    const int key_l = t * KT + sub0 + (FEW ? n : lane);
+    const uint64_t word = __ballot(key_l < len && (!mask || mask[key_l]));
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      const uint32_t word_u = (uint32_t)(word >> (FEW ? 0 : 32 * u));
+      if (!word_u && (DELTA || !p.ds)) continue;
+      const int at = (sub0 + 32 * u + n) * KS + M::E * h;
+      const f32x16 s = inner<T, DP>(ks + at, q, zero16());
+      f32x16 dp;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) dp[k] = -delta;
+      dp = inner<T, DP>(vs + at, g, dp);
+      const uint32_t w = word_u >> (4 * h);
+#pragma unroll
+      for (int run = 0; run < 4; ++run) {
+        const int key = t * KT + sub0 + 32 * u + 8 * run + 4 * h;
+        float bs[4], y[4];
+        if constexpr (BIAS) load_bias<T>(p, bias, key, row_ok, bias_vec, bs);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = 4 * run + e;
+          const float pr = exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[e]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
+          const bool seen = (w >> acc_row(k, 0)) & 1;
+          y[e] = seen ? pr * dp[k] : 0.f;
+          if constexpr (DELTA) sum += y[e];
+          dp[k] = SCALED<T> ? y[e] * sf : y[e];
+        }
+        if (ds) {
+          if (ds_vec && key < p.Lk) {
+            store4<float>(ds + key, y);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key + e < p.Lk) ds[key + e] = y[e];
+          }
+        }
+      }
+      if (!DELTA && word_u) M::template outer<DT>(ks + (sub0 + 32 * u) * KS, KS, lane, dp, dq);
+    }
+    __syncthreads();
+  }
+
+  if constexpr (DELTA) {
+    sum = xor32_sum(sum);
+    float* const to = p.part + (long)blk.z * p.B * p.H * p.Lq;
+    if constexpr (FEW) {
+      float* const part = reinterpret_cast<float*>(smem);   // [4][32]
+      if (h == 0) part[32 * wid + n] = sum;
+      __syncthreads();
+      if (threadIdx.x < 32 && row_ok) to[stat] = part[n] + part[32 + n] + part[64 + n] + part[96 + n];
+    } else if (h == 0 && row_ok) {
+      to[stat] = sum;
+    }
+    return;
+  }
+  const float out_scale = p.grad_scale / sf;
+  if constexpr (FEW) {
+    constexpr int OS = DP + 4;
+    float* const os = reinterpret_cast<float*>(smem);       // [4][32][OS]
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int run = 0; run < 4; ++run) {
+        const f32x4 v = {dq[dt][4 * run], dq[dt][4 * run + 1], dq[dt][4 * run + 2], dq[dt][4 * run + 3]};
+        *reinterpret_cast<f32x4*>(os + (32 * wid + n) * OS + 32 * dt + 8 * run + 4 * h) = v;
+      }
+    __syncthreads();
+    const int row = threadIdx.x >> 3, sub = threadIdx.x & 7, rr = blk.rt * ROWS + row;
+    if (rr >= p.rows) return;
+    const int ri = rr / p.G, rh = hk * p.G + rr - ri * p.G;
+    const long to = ((long)b * p.Lq + ri) * p.H + rh;
+    for (int d = 4 * sub; d < p.D; d += 32) {
+      float a[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) a[e] += os[(32 * w + row) * OS + d + e];
+        a[e] *= out_scale;
+      }
+      if (p.splits > 1) store4<float>(p.part + ((long)blk.z * p.B * p.Lq * p.H + to) * p.D + d, a);
+      else store4<T>((T*)p.dq + to * p.D + d, a);
+    }
+  } else {
+    if (!row_ok) return;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int run = 0; run < 4; ++run) {
+        const int d = 32 * dt + 8 * run + 4 * h;
+        if (d >= p.D) continue;
+        float a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = dq[dt][4 * run + e] * out_scale;
+        if (p.splits > 1) store4<float>(p.part + ((long)blk.z * p.B * p.Lq * p.H + row_at) * p.D + d, a);
+        else store4<T>((T*)p.dq + row_at * p.D + d, a);
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------ dk, dv
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256) void xa_dkv_kernel(XaParams p) {
+  using M = Mma<T>;
+  constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::row_stride(DP);
+  extern __shared__ __align__(16) char smem[];
+  T* const qs = reinterpret_cast<T*>(smem);
+  T* const gs = qs + RT * S;
+  float* const st = reinterpret_cast<float*>(gs + RT * S);   // [3][RT]: maximum, log2 of the sum, delta
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+  const Block blk = block_of(p, (p.Lk + XA_KEYS - 1) / XA_KEYS);
+  const int b = blk.b, hk = blk.hk;
+  const int key = blk.rt * XA_KEYS + 32 * wid + n;
+  const int len = length_of(p, b);
+  const uint8_t* mask = p.mask ? p.mask + b * p.mb : nullptr;
+  const bool seen = key < len && (!mask || mask[key]);
+  Frag<T, DP> kf, vf;
+  kf.load((const T*)p.k + b * p.kb + (long)key * p.kl + hk * p.kh, p.D, h, seen, p.neg);
+  vf.load((const T*)p.v + b * p.vb + (long)key * p.vl + hk * p.vh, p.D, h, seen);
+  const float sf = SCALED<T> ? ds_scale(p, b, hk) : 1.f;
+  constexpr float P_UP = SCALED<T> ? 15.f : 0.f, P_FACTOR = SCALED<T> ? 32768.f : 1.f;
+  const float ds_f = sf / P_FACTOR;
+  const bool any_seen = __any(seen);
+  // nothing of this workgroup's keys is seen by anyone: its sums are zero
+  const int t0 = blk.z * p.per, t1 = blk.rt * XA_KEYS < len ? min(t0 + p.per, (p.rows + RT - 1) / RT) : t0;
+
+  Stage<T, DP, RT> sq, sg;
+  float stat = 0.f;   // threads 0 .. 3 RT: one value of the tile's statistics
+  const int sw = threadIdx.x / RT, sr = threadIdx.x % RT;
+  auto load_tile = [&](int t) __attribute__((always_inline)) {
+    sq.load(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
+      const int r = t * RT + row;
+      if (r >= p.rows) return nullptr;
+      const int i = r / p.G, head = hk * p.G + r - i * p.G;
+      return (const T*)p.q + b * p.qb + i * p.ql + head * p.qh;
+    });
+    sg.load(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
+      const int r = t * RT + row;
+      if (r >= p.rows) return nullptr;
+      const int i = r / p.G, head = hk * p.G + r - i * p.G;
+      return (const T*)p.dout + (((long)b * p.Lq + i) * p.H + head) * p.D;
+    });
+    if (sw < 3) {
+      const int r = t * RT + sr;
+      stat = sw == 1 ? INFINITY : 0.f;   // a row behind the last: P = 0
+      if (r < p.rows) {
+        const int i = r / p.G, head = hk * p.G + r - i * p.G;
+        const long at = ((long)b * p.H + head) * p.Lq + i;
+        stat = sw == 0 ? p.st_m[at] : sw == 1 ? p.st_l[at] : p.delta[at];
+      }
+    }
+  };
+
+  const float c = BIAS ? p.scale : p.scale * LOG2E;
+  f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
+
+  if (t0 < t1) load_tile(t0);
+  for (int t = t0; t < t1; ++t) {
+    sq.store(qs, S);
+    sg.store(gs, S);
+    if (sw < 3) st[sw * RT + sr] = stat;
+    __syncthreads();
+    if (t + 1 < t1) load_tile(t + 1);
+    if (any_seen) {
+#pragma unroll
+      for (int u = 0; u < RT / 32; ++u) {
+        const int at = (32 * u + n) * S + M::E * h;
+        const f32x16 s = inner<T, DP>(qs + at, kf, zero16());
+        f32x16 pr, dp;
+#pragma unroll
+        for (int run = 0; run < 4; ++run) {
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(st + 2 * RT + 32 * u + 8 * run + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[4 * run + e] = -dl[e];
+        }
+        dp = inner<T, DP>(gs + at, vf, dp);
+#pragma unroll
+        for (int run = 0; run < 4; ++run) {
+          const f32x4 m = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * run + 4 * h);
+          const f32x4 ll = *reinterpret_cast<const f32x4*>(st + RT + 32 * u + 8 * run + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 4 * run + e;
+            float bs = 0.f;
+            if constexpr (BIAS) {
+              const int r = t * RT + 32 * u + acc_row(k, h);
+              if (r < p.rows && seen) {
+                const int i = r / p.G, head = hk * p.G + r - i * p.G;
+                const long ba = b * p.bb + head * p.bh + i * p.bq + key * p.bk;
+                bs = p.bias_f32 ? ((const float*)p.bias)[ba] : (float)((const T*)p.bias)[ba];
+              }
+            }
+            const float y = exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs) - m[e], LOG2E, P_UP - ll[e])
+                                           : exponent<T>(s[k], c, m[e]) + (P_UP - ll[e]));
+            pr[k] = seen ? y : 0.f;
+            dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
+          }
+        }
+        M::template outer<DT>(gs + 32 * u * S, S, lane, pr, dv);
+        M::template outer<DT>(qs + 32 * u * S, S, lane, dp, dk);
+      }
+    }
+    __syncthreads();
+  }
+
+  if (key >= p.Lk) return;
+  const float k_scale = p.grad_scale / sf, v_scale = 1.f / P_FACTOR;
+  const long at = ((long)b * p.Lk + key) * p.Hk + hk, all = (long)p.B * p.Lk * p.Hk;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int run = 0; run < 4; ++run) {
+      const int d = 32 * dt + 8 * run + 4 * h;
+      if (d >= p.D) continue;
+      float x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = seen ? dk[dt][4 * run + e] * k_scale : 0.f;
+        y[e] = seen ? dv[dt][4 * run + e] * v_scale : 0.f;
+      }
+      if (p.splits > 1) {
+        store4<float>(p.part + (2l * blk.z * all + at) * p.D + d, x);
+        store4<float>(p.part + ((2l * blk.z + 1) * all + at) * p.D + d, y);
+      } else {
+        store4<T>((T*)p.dk + at * p.D + d, x);
+        store4<T>((T*)p.dv + at * p.D + d, y);
+      }
+    }
+}
+
+// out = the sum over `splits` of part[z * step + e], four elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void xa_sum_kernel(const float* __restrict__ part, long step, int splits, T* __restrict__ out,
+                                                     long n) {
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= n) return;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (e + 3 >= n || step % 4) {   // statistics: any number of rows
+    for (int k = 0; k < 4 && e + k < n; ++k) {
+      for (int z = 0; z < splits; ++z) a[k] += part[z * step + e + k];
+      out[e + k] = (T)a[k];
+    }
+    return;
+  }
+#pragma unroll 4
+  for (int z = 0; z < splits; ++z) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(part + z * step + e);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] += v[k];
+  }
+  store4<T>(out + e, a);
+}
+
+template <typename T>
+int sum_launch(const float* part, long step, int splits, void* out, long n, hipStream_t st) {
+  xa_sum_kernel<T><<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(part, step, splits, (T*)out, n);
+  PF_CHECK_LAUNCH("xa_sum_kernel");
+  return PF_OK;
+}
+
+template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
+int dq_launch(const XaParams& p, hipStream_t st) {
+  constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
+  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * sizeof(T), join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0;
+  const size_t lds = tiles > join ? tiles : join;
+  if (int rc = pf_reserve_lds((const void*)xa_dq_kernel<T, DP, BIAS, FEW, DELTA>, lds, "xa_dq_kernel")) return rc;
+  const int rt = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
+  xa_dq_kernel<T, DP, BIAS, FEW, DELTA><<<(unsigned)((long)rt * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
+  PF_CHECK_LAUNCH("xa_dq_kernel");
+  if (p.splits == 1) return PF_OK;
+  const long rows = (long)p.B * p.Lq * p.H;
+  return DELTA ? sum_launch<float>(p.part, rows, p.splits, (float*)p.delta, rows, st)
+               : sum_launch<T>(p.part, rows * p.D, p.splits, p.dq, rows * p.D, st);
+}
+
+template <typename T, int DP>
+int dq_dp(const XaParams& p, hipStream_t st) {
+  if (p.bias) return p.few ? dq_launch<T, DP, true, true, false>(p, st) : dq_launch<T, DP, true, false, false>(p, st);
+  return p.few ? dq_launch<T, DP, false, true, false>(p, st) : dq_launch<T, DP, false, false, false>(p, st);
+}
+
+// delta of 16-bit types with a bias gradient (part: where the splits go, delta itself if there is one)
+template <typename T, int DP>
+int exact_delta_dp(const XaParams& p, hipStream_t st) {
+  return p.few ? dq_launch<T, DP, true, true, true>(p, st) : dq_launch<T, DP, true, false, true>(p, st);
+}
+
+template <typename T>
+int exact_delta_type(const XaParams& p, hipStream_t st) {
+  return p.D <= 32 ? exact_delta_dp<T, 32>(p, st) : p.D <= 64 ? exact_delta_dp<T, 64>(p, st) : exact_delta_dp<T, 128>(p, st);
+}
+
+template <typename T>
+int dq_type(const XaParams& p, hipStream_t st) {
+  return p.D <= 32 ? dq_dp<T, 32>(p, st) : p.D <= 64 ? dq_dp<T, 64>(p, st) : dq_dp<T, 128>(p, st);
+}
+
+template <typename T, int DP, bool BIAS>
+int dkv_launch(const XaParams& p, hipStream_t st) {
+  constexpr int RT = xa_rt(DP, __is_same(T, float));
+  const size_t lds = (size_t)2 * RT * Mma<T>::row_stride(DP) * sizeof(T) + 3 * RT * 4;
+  if (int rc = pf_reserve_lds((const void*)xa_dkv_kernel<T, DP, BIAS>, lds, "xa_dkv_kernel")) return rc;
+  const int tiles = (p.Lk + XA_KEYS - 1) / XA_KEYS;
+  xa_dkv_kernel<T, DP, BIAS><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
+  PF_CHECK_LAUNCH("xa_dkv_kernel");
+  if (p.splits == 1) return PF_OK;
+  const long n = (long)p.B * p.Lk * p.Hk * p.D;
+  if (int rc = sum_launch<T>(p.part, 2 * n, p.splits, p.dk, n, st)) return rc;
+  return sum_launch<T>(p.part + n, 2 * n, p.splits, p.dv, n, st);
+}
+
+template <typename T, int DP>
+int dkv_dp(const XaParams& p, hipStream_t st) {
+  return p.bias ? dkv_launch<T, DP, true>(p, st) : dkv_launch<T, DP, false>(p, st);
+}
+
+template <typename T>
+int dkv_type(const XaParams& p, hipStream_t st) {
+  return p.D <= 32 ? dkv_dp<T, 32>(p, st) : p.D <= 64 ? dkv_dp<T, 64>(p, st) : dkv_dp<T, 128>(p, st);
+}
+
+template <typename T>
+int delta_type(const XaParams& p, float* delta, uint32_t* amax, hipStream_t st) {
+  const long rows = (long)p.B * p.Lq * p.H + (SCALED<T> ? (long)p.B * p.Lk * p.Hk : 0);
+  xa_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(p, delta, amax);
+  PF_CHECK_LAUNCH("xa_delta_kernel");
+  return PF_OK;
+}
+
+}  // namespace

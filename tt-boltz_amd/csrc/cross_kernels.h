@@ -1,0 +1,488 @@
+// Cross attention kernels, included once per element type T (see cross_attn.h).
+//
+//   x_ij = scale q_i . k_j + bias_ij, -inf where key j is hidden;  P = softmax_j(x);  o_i = sum_j P_ij v_j
+//   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (do_i . v_j - delta_i),  delta_i = do_i . o_i,
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dbias = dS
+//
+// Every product runs on 32x32 MFMA tiles (accumulators: lane l, register r hold column l & 31, row
+// 8 (r >> 2) + 4 (l >> 5) + (r & 3)).  The forward and the dq kernel form S^T = K Q^T, so a lane's
+// column is one query: its softmax statistics are the lane's own, and the accumulator of P^T (dS^T)
+// is, as it stands, the right operand of O^T = V^T P^T (dQ^T = K^T dS^T), with the left operand read
+// from LDS in the accumulators' key order.  The dk, dv kernel forms S = Q K^T: its lanes hold keys.
+//
+// Heads that share a key head are rows of one tile, so keys and values are read once for them.
+#pragma once
+#include "cross_attn.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int V>
+struct IntC { static constexpr int value = V; };
+
+PF_DEV f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+PF_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+PF_DEV float xor32_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+PF_DEV float xor32_sum(float v) { return v + __shfl_xor(v, 32); }
+PF_DEV int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// ------------------------------------------------------------------------------ tiles
+// Frag<DP>: 32 rows x DP channels as an MFMA operand of products over channels.  Lane (n, h) holds of
+// row n, per step s, the 16 bytes at channel CH s + h * CH / 2 (CH channels a step: 16 of 16 bits,
+// 8 fp32; the two halves of the wave hold the step's two halves).
+template <typename T>
+struct Mma {
+  typedef T frag_t __attribute__((ext_vector_type(8)));
+  typedef T quad_t __attribute__((ext_vector_type(4)));
+  static constexpr int CH = 16, E = 8;
+  static constexpr int row_stride(int dp) { return dp + 8; }   // rows land on distinct banks (16 lanes x 16 bytes)
+  // only read in transposed 4 x 16 blocks: four rows x 32 channels on distinct banks
+  static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp + 32; }
+  static PF_DEV f32x16 mma(const frag_t& a, const frag_t& b, const f32x16& c) {
+    if constexpr (__is_same(T, half_t)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // acc[dt] += X^T p over 32 rows of the LDS tile X (row stride `st`): p is an accumulator, and X's
+  // rows are taken in its order.  A transposing read hands lane i of 16 the column i of a 4 x 16 block
+  // whose 8-byte pieces the lanes point at.
+  template <int DT>
+  static PF_DEV void outer(const T* x, int st, int lane, const f32x16& p, f32x16 (&acc)[DT]) {
+    const int h = lane >> 5, i = lane & 15, c16 = (lane >> 4) & 1;
+    const T* at = x + (4 * h + (i >> 2)) * st + 16 * c16 + 4 * (i & 3);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      frag_t b;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) b[t] = (T)p[8 * s + t];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const quad_t lo = tr_read(at + (16 * s) * st + 32 * dt), hi = tr_read(at + (16 * s + 8) * st + 32 * dt);
+        const frag_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[dt] = mma(a, b, acc[dt]);
+      }
+    }
+  }
+  static PF_DEV quad_t tr_read(const T* p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_t;
+    return __builtin_bit_cast(quad_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p));
+  }
+};
+
+template <>
+struct Mma<float> {
+  typedef f32x4 frag_t;
+  static constexpr int CH = 8, E = 4;
+  static constexpr int row_stride(int dp) { return dp + 4; }
+  static constexpr int col_stride(int dp) { return dp + 4; }
+  static PF_DEV f32x16 mma(const frag_t& a, const frag_t& b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  template <int DT>
+  static PF_DEV void outer(const float* x, int st, int lane, const f32x16& p, f32x16 (&acc)[DT]) {
+    const int h = lane >> 5, n = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[acc_row(r, h) * st + 32 * dt + n], p[r], acc[dt], 0, 0, 0);
+  }
+};
+
+template <typename T, int DP>
+struct Frag {
+  static constexpr int S = DP / Mma<T>::CH;
+  typename Mma<T>::frag_t f[S];
+  // row `p` in global memory; channels >= D are zero, and all are where !ok
+  PF_DEV void load(const T* p, int D, int h, bool ok, bool neg = false) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int d = Mma<T>::CH * s + Mma<T>::E * h;
+      typename Mma<T>::frag_t z = {};
+      f[s] = ok && d < D ? *reinterpret_cast<const typename Mma<T>::frag_t*>(p + d) : z;
+      if (neg) f[s] = -f[s];
+    }
+  }
+};
+
+// c += A B^T over channels: A the LDS tile's 32 rows at `a` (this lane's row, channel E h), B a fragment
+template <typename T, int DP>
+PF_DEV f32x16 inner(const T* a, const Frag<T, DP>& b, f32x16 c) {
+#pragma unroll
+  for (int s = 0; s < Frag<T, DP>::S; ++s)
+    c = Mma<T>::mma(*reinterpret_cast<const typename Mma<T>::frag_t*>(a + Mma<T>::CH * s), b.f[s], c);
+  return c;
+}
+
+// A tile of ROWS rows x DP channels on its way from global memory to LDS: 16-byte pieces in registers.
+template <typename T, int DP, int ROWS>
+struct Stage {
+  typedef typename Vec16<T>::type vec_t;
+  static constexpr int N = Vec16<T>::N, PER = DP / N, CH = ROWS * PER / 256;
+  static_assert(ROWS * PER % 256 == 0, "whole pieces per thread");
+  vec_t v[CH];
+  // row(r): the row's address, or null (zeros)
+  template <typename F>
+  PF_DEV void load(int D, F row) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int c = threadIdx.x + 256 * j, r = c / PER, d = (c % PER) * N;
+      const T* p = row(r);
+      vec_t z = {};
+      v[j] = p && d < D ? *reinterpret_cast<const vec_t*>(p + d) : z;
+    }
+  }
+  PF_DEV void store(T* lds, int stride) const {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int c = threadIdx.x + 256 * j, r = c / PER, d = (c % PER) * N;
+      *reinterpret_cast<vec_t*>(lds + r * stride + d) = v[j];
+    }
+  }
+};
+
+// Consecutive workgroups of one (batch, key head) on one XCD: its keys and values stay in that L2.
+PF_DEV int xcd_remap(int w, int total) { return total % 8 ? w : (w % 8) * (total / 8) + w / 8; }
+
+struct Block { int rt, z, b, hk; };
+PF_DEV Block block_of(const XaParams& p, int tiles) {
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int rt = id % tiles, rest = id / tiles, z = rest % p.splits, bh = rest / p.splits;
+  return {rt, z, bh / p.Hk, bh % p.Hk};
+}
+
+PF_DEV int length_of(const XaParams& p, int b) { return p.lens ? max(0, min(p.Lk, p.lens[b])) : p.Lk; }
+
+// bias[row, key .. key + 3] of a lane's query (0 outside the tensor)
+template <typename T>
+PF_DEV void load_bias(const XaParams& p, const char* row, int key, bool ok, bool vec, float (&x)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = 0.f;
+  if (!ok || key >= p.Lk) return;
+  if (p.bias_f32) {
+    const float* a = reinterpret_cast<const float*>(row);
+    if (vec && key + 3 < p.Lk) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a + key);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (key + e < p.Lk) x[e] = a[(key + e) * p.bk];
+    }
+  } else {
+    const T* a = reinterpret_cast<const T*>(row);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (key + e < p.Lk) x[e] = (float)a[(key + e) * p.bk];
+  }
+}
+
+// c s - m, the exponent of a probability without a bias.  fp32 tensors: the product is rounded before
+// the difference, so the largest logit gives exactly 0 (a query that sees one key gets that value, bit
+// for bit); of 16-bit tensors one fused step is as good (2^-24 of the logit) and half the work.
+template <typename T>
+PF_DEV float exponent(float s, float c, float m) {
+  if constexpr (__is_same(T, float)) {
+#pragma clang fp contract(off)
+    const float x = s * c;
+    return x - m;
+  } else {
+    return fmaf(s, c, -m);
+  }
+}
+
+// 4 consecutive results of a row
+template <typename T>
+PF_DEV void store4(T* p, const float (&x)[4]) {
+  typedef T quad __attribute__((ext_vector_type(4)));
+  quad v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (T)x[e];
+  *reinterpret_cast<quad*>(p) = v;
+}
+
+// ------------------------------------------------------------------------------ forward
+// FEW = false: 4 waves x 32 rows, every wave over the tile's 64 keys.  FEW = true (at most 32 rows, and
+// few enough tiles): the waves share a 32-row tile and take 32 of the tile's 128 keys each; their
+// results are joined through LDS.
+template <typename T, int DP, bool BIAS, bool FEW>
+__global__ __launch_bounds__(256) void xa_fwd_kernel(XaParams p) {
+  using M = Mma<T>;
+  constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
+  constexpr int KS = M::row_stride(DP), VS = M::col_stride(DP);
+  extern __shared__ __align__(16) char smem[];
+  T* const ks = reinterpret_cast<T*>(smem);
+  T* const vs = ks + KT * KS;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+  constexpr int ROWS = FEW ? 32 : 128;
+  const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
+  const int b = blk.b, hk = blk.hk;
+  const int r = blk.rt * ROWS + (FEW ? 0 : 32 * wid) + n;
+  const bool row_ok = r < p.rows;
+  const int i = row_ok ? r / p.G : 0, head = hk * p.G + (row_ok ? r - i * p.G : 0);
+  const int sub0 = FEW ? 32 * wid : 0;
+  Frag<T, DP> q;
+  q.load((const T*)p.q + b * p.qb + i * p.ql + head * p.qh, p.D, h, row_ok, p.neg);
+  const char* bias = nullptr;
+  bool bias_vec = false;
+  if constexpr (BIAS) {
+    const long at = b * p.bb + head * p.bh + i * p.bq;
+    bias = (const char*)p.bias + at * (p.bias_f32 ? 4 : (long)sizeof(T));
+    bias_vec = p.bk == 1 && ((p.bb | p.bh | p.bq) & 3) == 0 && ((uintptr_t)p.bias & 15) == 0;
+  }
+  const int len = length_of(p, b);
+  const int t0 = blk.z * p.per, t1 = min(t0 + p.per, (len + KT - 1) / KT);
+  const uint8_t* mask = p.mask ? p.mask + b * p.mb : nullptr;
+  const T* const kb = (const T*)p.k + b * p.kb + hk * p.kh;
+  const T* const vb = (const T*)p.v + b * p.vb + hk * p.vh;
+
+  Stage<T, DP, KT> sk, sv;
+  auto load_tile = [&](int t) __attribute__((always_inline)) {
+    // a hidden key's rows are zeros: what stands there (NaN, say) takes no part
+    auto seen = [&](int row) __attribute__((always_inline)) {
+      const int key = t * KT + row;
+      return key < len && (!mask || mask[key]);
+    };
+    sk.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? kb + (long)(t * KT + row) * p.kl : nullptr; });
+    sv.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? vb + (long)(t * KT + row) * p.vl : nullptr; });
+  };
+
+  const float c = BIAS ? p.scale : p.scale * LOG2E;   // x in units of 1 (bias) or log2
+  float m = -INFINITY, l = 0.f;                       // l: this lane's half of the keys
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
+
+  if (t0 < t1) load_tile(t0);
+  for (int t = t0; t < t1; ++t) {
+    sk.store(ks, KS);
+    sv.store(vs, VS);
+    __syncthreads();
+    if (t + 1 < t1) load_tile(t + 1);
+    // the keys of this wave that are seen, bit j: key sub0 + j of the tile
+    const int key_l = t * KT + sub0 + (FEW ? n : lane);
+    const uint64_t word = __ballot(key_l < len && (!mask || mask[key_l]));
+    if (word) {
+      float x[NSUB][16];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u) {
+        const f32x16 s = inner<T, DP>(ks + (sub0 + 32 * u + n) * KS + M::E * h, q, zero16());
+#pragma unroll
+        for (int run = 0; run < 4; ++run) {
+          float bs[4];
+          if constexpr (BIAS) load_bias<T>(p, bias, t * KT + sub0 + 32 * u + 8 * run + 4 * h, row_ok, bias_vec, bs);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][4 * run + e] = BIAS ? fmaf(s[4 * run + e], c, bs[e]) : s[4 * run + e];
+        }
+        const uint32_t w = (uint32_t)(word >> (FEW ? 0 : 32 * u)) >> (4 * h);
+        if ((uint32_t)(word >> (FEW ? 0 : 32 * u)) != 0xffffffffu) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[u][k] = (w >> acc_row(k, 0)) & 1 ? x[u][k] : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, x[u][k]);
+      }
+      mx = xor32_max(mx);
+      const float m_new = fmaxf(m, BIAS ? mx : mx * c);
+      if (__any(m_new > m)) {
+        const float a = m_new > m ? exp2_fast(BIAS ? (m - m_new) * LOG2E : m - m_new) : 1.f;
+        l *= a;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[dt][k] *= a;
+        m = m_new;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;   // nothing seen so far: every p is 0
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u) {
+        f32x16 pr;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          pr[k] = exp2_fast(BIAS ? (x[u][k] - mu) * LOG2E : exponent<T>(x[u][k], c, mu));
+          l += pr[k];
+        }
+        M::template outer<DT>(vs + (sub0 + 32 * u) * VS, VS, lane, pr, o);
+      }
+    }
+    __syncthreads();
+  }
+  l = xor32_sum(l);
+
+  if constexpr (FEW) {
+    // join the four waves: their maxima and sums, then thread (row, 4 channels) adds the four parts
+    constexpr int OS = DP + 4;
+    float* const os = reinterpret_cast<float*>(smem);       // [4][32][OS]
+    float* const ms = os + 4 * 32 * OS;                     // [4][32][2]
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int run = 0; run < 4; ++run) {
+        const f32x4 v = {o[dt][4 * run], o[dt][4 * run + 1], o[dt][4 * run + 2], o[dt][4 * run + 3]};
+        *reinterpret_cast<f32x4*>(os + (32 * wid + n) * OS + 32 * dt + 8 * run + 4 * h) = v;
+      }
+    if (h == 0) {
+      ms[(32 * wid + n) * 2] = m;
+      ms[(32 * wid + n) * 2 + 1] = l;
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 3, sub = threadIdx.x & 7, rr = blk.rt * ROWS + row;
+    if (rr >= p.rows) return;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ms[(32 * w + row) * 2]);
+    float f[4], ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = ms[(32 * w + row) * 2];
+      f[w] = mw == -INFINITY ? 0.f : exp2_fast(BIAS ? (mw - mm) * LOG2E : mw - mm);
+      ll += f[w] * ms[(32 * w + row) * 2 + 1];
+    }
+    // (a wave that saw nothing has sums of 0, or NaN where its scores were: they must spread)
+    const int ri = rr / p.G, rh = hk * p.G + rr - ri * p.G;
+    const long row_at = ((long)b * p.Lq + ri) * p.H + rh;
+    const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+    const long part_row = ((long)blk.z * p.B * p.Hk + (long)b * p.Hk + hk) * p.rows + rr;
+    const long part_rows = (long)p.splits * p.B * p.Hk * p.rows;
+    for (int d = 4 * sub; d < p.D; d += 32) {
+      float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += f[w] * os[(32 * w + row) * OS + d + e];
+      if (p.splits > 1) {
+        store4<float>(p.part + part_row * p.D + d, a);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] *= inv;
+      store4<T>((T*)p.o + row_at * p.D + d, a);
+      if (p.o32) store4<float>(p.o32 + row_at * p.D + d, a);
+    }
+    if (sub == 0) {
+      if (p.splits > 1) {
+        p.part[part_rows * p.D + 2 * part_row] = mm;
+        p.part[part_rows * p.D + 2 * part_row + 1] = ll;
+      } else if (p.st_m) {
+        const long at = ((long)b * p.H + rh) * p.Lq + ri;
+        p.st_m[at] = mm == -INFINITY ? 0.f : mm;
+        p.st_l[at] = ll == 0.f ? INFINITY : __builtin_amdgcn_logf(ll);
+      }
+    }
+  } else {
+    if (!row_ok) return;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const long row_at = ((long)b * p.Lq + i) * p.H + head;
+    const long part_row = ((long)blk.z * p.B * p.Hk + (long)b * p.Hk + hk) * p.rows + r;
+    const long part_rows = (long)p.splits * p.B * p.Hk * p.rows;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int run = 0; run < 4; ++run) {
+        const int d = 32 * dt + 8 * run + 4 * h;
+        if (d >= p.D) continue;
+        float a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = o[dt][4 * run + e] * (p.splits > 1 ? 1.f : inv);
+        if (p.splits > 1) {
+          store4<float>(p.part + part_row * p.D + d, a);
+        } else {
+          store4<T>((T*)p.o + row_at * p.D + d, a);
+          if (p.o32) store4<float>(p.o32 + row_at * p.D + d, a);
+        }
+      }
+    if (h == 0) {
+      if (p.splits > 1) {
+        p.part[part_rows * p.D + 2 * part_row] = m;
+        p.part[part_rows * p.D + 2 * part_row + 1] = l;
+      } else if (p.st_m) {
+        const long at = ((long)b * p.H + head) * p.Lq + i;
+        p.st_m[at] = m == -INFINITY ? 0.f : m;
+        p.st_l[at] = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+      }
+    }
+  }
+}
+
+// The splits of a row joined: a thread for 4 channels.
+template <typename T, bool BIAS>
+__global__ __launch_bounds__(256) void xa_join_kernel(XaParams p) {
+  const int per = p.D / 4;
+  const long e = (long)blockIdx.x * 256 + threadIdx.x;
+  const long row = e / per;   // (b, hk, r)
+  const int d = (int)(e - row * per) * 4;
+  const long all = (long)p.B * p.Hk * p.rows;
+  if (row >= all) return;
+  const float* ml = p.part + all * p.splits * p.D;
+  float mm = -INFINITY;
+  for (int z = 0; z < p.splits; ++z) mm = fmaxf(mm, ml[2 * (z * all + row)]);
+  float l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int z = 0; z < p.splits; ++z) {
+    const float mz = ml[2 * (z * all + row)];
+    const float f = mz == -INFINITY ? 0.f : exp2_fast(BIAS ? (mz - mm) * LOG2E : mz - mm);
+    l += f * ml[2 * (z * all + row) + 1];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p.part + (z * all + row) * p.D + d);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] += f * v[k];
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] *= inv;
+  const long bh = row / p.rows;
+  const int r = (int)(row - bh * p.rows), i = r / p.G, b = (int)(bh / p.Hk), head = (int)(bh % p.Hk) * p.G + r - i * p.G;
+  const long at = (((long)b * p.Lq + i) * p.H + head) * p.D + d;
+  store4<T>((T*)p.o + at, a);
+  if (p.o32) store4<float>(p.o32 + at, a);
+  if (d == 0 && p.st_m) {
+    const long s = ((long)b * p.H + head) * p.Lq + i;
+    p.st_m[s] = mm == -INFINITY ? 0.f : mm;
+    p.st_l[s] = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+  }
+}
+
+template <typename T, int DP, bool FEW>
+size_t fwd_lds() {
+  constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
+  const size_t tiles = (size_t)KT * (Mma<T>::row_stride(DP) + Mma<T>::col_stride(DP)) * sizeof(T);
+  const size_t join = FEW ? (size_t)4 * 32 * (DP + 4 + 2) * 4 : 0;
+  return tiles > join ? tiles : join;
+}
+
+template <typename T, int DP, bool BIAS, bool FEW>
+int fwd_launch(const XaParams& p, hipStream_t st) {
+  const size_t lds = fwd_lds<T, DP, FEW>();
+  if (int rc = pf_reserve_lds((const void*)xa_fwd_kernel<T, DP, BIAS, FEW>, lds, "xa_fwd_kernel")) return rc;
+  const int tiles = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
+  xa_fwd_kernel<T, DP, BIAS, FEW><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
+  PF_CHECK_LAUNCH("xa_fwd_kernel");
+  if (p.splits > 1) {
+    const long threads = (long)p.B * p.Hk * p.rows * (p.D / 4);
+    xa_join_kernel<T, BIAS><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(p);
+    PF_CHECK_LAUNCH("xa_join_kernel");
+  }
+  return PF_OK;
+}
+
+template <typename T, int DP>
+int fwd_dp(const XaParams& p, hipStream_t st) {
+  if (p.bias) return p.few ? fwd_launch<T, DP, true, true>(p, st) : fwd_launch<T, DP, true, false>(p, st);
+  return p.few ? fwd_launch<T, DP, false, true>(p, st) : fwd_launch<T, DP, false, false>(p, st);
+}
+
+template <typename T>
+int fwd_type(const XaParams& p, hipStream_t st) {
+  return p.D <= 32 ? fwd_dp<T, 32>(p, st) : p.D <= 64 ? fwd_dp<T, 64>(p, st) : fwd_dp<T, 128>(p, st);
+}
+
+}  // namespace

@@ -799,6 +799,7 @@ def launch_msa_embed(msa: torch.Tensor, has_deletion: Optional[torch.Tensor], de
 
 # operators between tracks, in the caller's own element type
 from .track_ops import (  # noqa: E402,F401
-    dropout_add, embedding, embedding_grad, embedding_grad_workspace_bytes, launch_dropout_add, launch_embedding,
-    launch_embedding_grad,
+    cross_attention, cross_attention_bwd_workspace_bytes, cross_attention_workspace_bytes, dropout_add, embedding,
+    embedding_grad, embedding_grad_workspace_bytes, launch_cross_attention, launch_cross_attention_bwd,
+    launch_dropout_add, launch_embedding, launch_embedding_grad,
 )

@@ -1,9 +1,9 @@
 """Operators between tracks in the caller's own element type, with their gradients.
 
-``embedding`` (token -> atom broadcasts, residue types, vocabularies) with ``embedding_grad`` (its
+``cross_attention`` (queries of one track over another track's keys and values), ``embedding`` (token -> atom broadcasts, residue types, vocabularies) with ``embedding_grad`` (its
 transpose: sums by token) and ``dropout_add`` (the pair updates' residual dropout) take fp32, fp16 or
 bf16 device tensors and return the same type; sums and statistics are fp32.  They differentiate like
-torch's own operators (first derivatives).  The ``launch_*`` functions enqueue the kernels on the
+torch's own operators (``cross_attention`` once).  The ``launch_*`` functions enqueue the kernels on the
 current stream, for programs that write their own backward pass or capture one: they take contiguous
 device tensors and allocate nothing.
 
@@ -16,8 +16,9 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 import operator
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -61,6 +62,197 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# --------------------------------------------------------------------------------------
+# cross attention
+# --------------------------------------------------------------------------------------
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    """``t`` where the kernels can read it in 16-byte pieces of its last dimension, else a copy."""
+    t = t.detach()
+    unit = 16 // t.element_size()
+    if (t.is_neg() or t.data_ptr() % 16 or (t.shape[-1] > 1 and t.stride(-1) != 1)
+            or any(s % unit for n, s in zip(t.shape[:-1], t.stride()) if n > 1)):
+        t = t.resolve_neg().clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = _dense(t)
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _strides(t: torch.Tensor, dims) -> list:
+    return [t.stride(d) if t.shape[d] > 1 else 0 for d in dims]
+
+
+def _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats) -> "_lib.CrossAttnArgs":
+    (B, Lq, H, D), (_, Lk, Hk, _) = q.shape, k.shape
+    a = _lib.CrossAttnArgs(B, Lq, Lk, H, Hk, D, DTYPE_CODE[q.dtype], 0 if bias is None else DTYPE_CODE[bias.dtype], scale,
+                           q.data_ptr(), *_strides(q, (0, 1, 2)), k.data_ptr(), *_strides(k, (0, 1, 2)),
+                           v.data_ptr(), *_strides(v, (0, 1, 2)))
+    if bias is not None:
+        a.bias = bias.data_ptr()
+        a.bias_b, a.bias_h, a.bias_q, a.bias_k = _strides(bias, (0, 1, 2, 3))
+        if Lk == 1:
+            a.bias_k = 1
+    if mask is not None:
+        a.mask, a.mask_b = mask.data_ptr(), mask.stride(0) if B > 1 else 0
+    a.k_lens, a.o, a.o32, a.stats = ops._ptr(k_lens), ops._ptr(o), ops._ptr(o32), ops._ptr(stats)
+    return a
+
+
+def launch_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                           bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                           k_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                           o32: Optional[torch.Tensor] = None, stats: Optional[torch.Tensor] = None,
+                           ws: Optional[torch.Tensor] = None) -> None:
+    """o = cross attention (pf_cross_attn_fwd) of q [B, Lq, H, D] on k, v [B, Lk, Hk, D]; bias
+    [B or 1, H or 1, Lq, Lk], mask bool or uint8 [B, Lk], k_lens int32 [B].  ``o32`` fp32 like o (16-bit
+    types) and ``stats`` fp32 [2, B, H, Lq] keep what the backward pass needs; ``ws`` of
+    ``cross_attention_workspace_bytes``.  (With a bias gradient, 16-bit types need no ``o32``.)"""
+    a = _cross_args(q, k, v, bias, mask, k_lens, q.shape[-1] ** -0.5 if scale is None else scale, o, o32, stats)
+    a.workspace, a.workspace_bytes, a.stream = ops._ptr(ws), 0 if ws is None else ws.numel(), ops._stream()
+    _lib.check(_lib.load().pf_cross_attn_fwd(ctypes.byref(a)), "pf_cross_attn_fwd")
+
+
+def cross_attention_workspace_bytes(q: torch.Tensor, k: torch.Tensor) -> int:
+    return _lib.load().pf_cross_attn_workspace_size(ctypes.byref(_cross_args(q, k, k, None, None, None, 1.0, None, None, None)))
+
+
+def _bwd_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats, dbias_shape):
+    a = _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats)
+    if dbias_shape is not None:
+        a.dbias_B, a.dbias_H = dbias_shape[:2]
+    return a
+
+
+def cross_attention_bwd_workspace_bytes(q: torch.Tensor, k: torch.Tensor, bias: Optional[torch.Tensor] = None) -> int:
+    """``bias``: the bias whose gradient is wanted, or None."""
+    a = _bwd_args(q, k, k, bias, None, None, 1.0, None, None, None, None if bias is None else bias.shape)
+    return _lib.load().pf_cross_attn_bwd_workspace_size(ctypes.byref(a))
+
+
+def launch_cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                               o: torch.Tensor, o32: Optional[torch.Tensor], stats: torch.Tensor,
+                               dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv: Optional[torch.Tensor],
+                               ws: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                               dbias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                               k_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> None:
+    """The gradients of ``launch_cross_attention`` (pf_cross_attn_bwd) into contiguous dq, dk, dv and
+    dbias (of bias's shape and type); dq alone, or dk and dv alone, where the others are None."""
+    a = _bwd_args(q, k, v, bias, mask, k_lens, q.shape[-1] ** -0.5 if scale is None else scale, o, o32, stats,
+                  None if dbias is None else dbias.shape)
+    a.dout, a.dq, a.dk, a.dv, a.dbias = ops._ptr(do), ops._ptr(dq), ops._ptr(dk), ops._ptr(dv), ops._ptr(dbias)
+    a.workspace, a.workspace_bytes, a.stream = ops._ptr(ws), ws.numel(), ops._stream()
+    _lib.check(_lib.load().pf_cross_attn_bwd(ctypes.byref(a)), "pf_cross_attn_bwd")
+
+
+def _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep: bool, keep_o: bool = False):
+    """(o, o32, stats) on prepared tensors; the last two only where a backward pass will read them."""
+    dev = q.device
+    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    o32 = torch.empty(q.shape, dtype=torch.float32, device=dev) if keep_o and q.dtype != torch.float32 else None
+    stats = torch.empty((2, q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if keep else None
+    with _on(dev):
+        nb = cross_attention_workspace_bytes(q, k)
+        launch_cross_attention(q, k, v, o, bias, mask, k_lens, scale, o32, stats, ops.workspace(nb, dev) if nb else None)
+    return o, o32, stats
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, mask, k_lens, scale):
+        qs, ks, vs = _strided(q), _strided(k), _strided(v)
+        b = None if bias is None else bias.detach()
+        # (a bias gradient of 16-bit types does without the unrounded o)
+        o, o32, stats = _cross_fwd(qs, ks, vs, b, mask, k_lens, scale, True, not ctx.needs_input_grad[3])
+        ctx.save_for_backward(q, k, v, bias, mask, k_lens, o if q.dtype == torch.float32 else o32, stats)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, bias, mask, k_lens, o32, stats = ctx.saved_tensors
+        want_q, want_k, want_v, want_b = ctx.needs_input_grad[:4]
+        q, k, v, do = _strided(q), _strided(k), _strided(v), _aligned(grad)
+        bias = None if bias is None else bias.detach()
+        dev = q.device
+        some = q.numel() > 0 and k.numel() > 0   # else nothing is launched, and what has elements is zero
+        make = torch.empty if some else torch.zeros
+        dq = make(q.shape, dtype=q.dtype, device=dev) if want_q or want_b else None
+        dk, dv = (make(k.shape, dtype=q.dtype, device=dev) if want_k or want_v else None for _ in range(2))
+        dbias = make(bias.shape, dtype=bias.dtype, device=dev) if want_b else None
+        if some:
+            with _on(dev):
+                ws = ops.workspace(cross_attention_bwd_workspace_bytes(q, k, bias if want_b else None), dev)
+                launch_cross_attention_bwd(do, q, k, v, o32, o32, stats, dq, dk, dv, ws, bias, dbias, mask, k_lens, ctx.scale)
+        return dq if want_q else None, dk if want_k else None, dv if want_v else None, dbias, None, None, None
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                    mask: Optional[torch.Tensor] = None, k_lens: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of one track's queries over another track's keys and values:
+    ``softmax_j(scale q_i . k_j + bias_ij) v_j``, as ``AttentionPairBias`` with keys of another length
+    (``tt_bio/boltz2.py:343-367``: atom windows, tokens against atoms) or a decoder over an encoder's
+    states.  Returns [B, Lq, H, D] in q's type; differentiable in q, k, v and bias.
+
+    q: [B, Lq, H, D]; k, v: [B, Lk, Hk, D], H a multiple of Hk (each key head serves H / Hk query heads in
+    a row), all fp32, fp16 or bf16, D a multiple of 8 up to 128; views of any strides are read in place
+    where 16-byte pieces allow it (a batch of beams may share states through ``expand``).
+    bias: added to the logits, [B or 1, H or 1, Lq, Lk] (leading dimensions may be missing), fp32 or q's
+    type; -inf hides a key from a query.  mask: [B, Lk] (or [1, Lk], [Lk]), bool or numbers, keys of 0 are
+    hidden; k_lens: int32 or int64 [B], keys from k_lens[b] on are hidden (lengths outside [0, Lk] count as
+    the nearer end).  Hidden keys are not used, whatever they hold; a query that sees nothing gives zeros.
+    scale: D ** -0.5 by default.
+
+    Softmax statistics and sums are fp32; 16-bit types round P (and in the backward pass dS) to their type
+    for the products, fp32 runs on fp32 products throughout."""
+    _device("cross_attention", q, k, v, bias, mask, k_lens)
+    _code("cross_attention", q)
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"cross_attention expects q [B, Lq, H, D] and k, v [B, Lk, Hk, D], got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hk == 0 or H % Hk:
+        raise ValueError(f"cross_attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)} "
+                         "([B, Lk, Hk, D], H a multiple of Hk)")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"cross_attention: q, k and v differ in type ({q.dtype}, {k.dtype}, {v.dtype})")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"cross_attention: D must be a multiple of 8 up to 128, got {D}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale) or abs(scale) > 3e38:
+        raise ValueError(f"cross_attention: scale must be finite, got {scale}")
+    if bias is not None:
+        if bias.dim() > 4 or bias.dim() < 2:
+            raise ValueError(f"cross_attention expects bias [B or 1, H or 1, Lq, Lk], got {tuple(bias.shape)}")
+        bias = bias[(None,) * (4 - bias.dim())]
+        if bias.shape[0] not in (1, B) or bias.shape[1] not in (1, H) or tuple(bias.shape[2:]) != (Lq, Lk):
+            raise ValueError(f"cross_attention: bias {tuple(bias.shape)} does not fit [{B} or 1, {H} or 1, {Lq}, {Lk}]")
+        if bias.dtype not in (torch.float32, q.dtype):
+            raise ValueError(f"cross_attention: bias is {bias.dtype} (fp32 or {q.dtype} is needed)")
+        if bias.is_neg():
+            bias = bias.resolve_neg()
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            mask = mask.detach() != 0
+        mask = ops.shaped(mask, (B, Lk))
+        if Lk > 1 and mask.stride(1) != 1:
+            mask = mask.contiguous()
+    if k_lens is not None:
+        if k_lens.dtype not in (torch.int32, torch.int64) or tuple(k_lens.shape) != (B,):
+            raise ValueError(f"cross_attention expects k_lens int32 or int64 [{B}], got {k_lens.dtype} {tuple(k_lens.shape)}")
+        if k_lens.dtype == torch.int64:
+            k_lens = k_lens.clamp(0, Lk).to(torch.int32)
+        k_lens = k_lens.contiguous()
+    if _wants_grad(q, k, v, bias):
+        return _CrossAttention.apply(q, k, v, bias, mask, k_lens, scale)
+    return _cross_fwd(_strided(q), _strided(k), _strided(v), None if bias is None else bias.detach(), mask, k_lens, scale,
+                      False)[0]
 
 
 # --------------------------------------------------------------------------------------
@@ -114,7 +306,6 @@ class _Embedding(torch.autograd.Function):
         return _embedding(index, weight, scale)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         index, = ctx.saved_tensors
         return None, embedding_grad(grad, index, ctx.rows, ctx.scale), None
@@ -128,7 +319,7 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> 
     Differentiable in ``weight``; see :func:`embedding_grad`.  The lookup in place of a one-hot
     product, as ``MSA`` embeds its alignment (``tt_bio/reference.py:1253-1276``) and the atom
     transformer broadcasts token states."""
-    dev = _device("embedding", index, weight)
+    _device("embedding", index, weight)
     if weight.dim() != 2:
         raise ValueError(f"embedding expects weight [V, C], got {tuple(weight.shape)}")
     _code("embedding", weight)
@@ -138,13 +329,37 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> 
     return _embedding(index, weight, float(scale))
 
 
+def _embedding_grad(grad: torch.Tensor, index: torch.Tensor, num_rows: int, scale: float) -> torch.Tensor:
+    grad = _dense(grad)
+    C = grad.shape[-1]
+    dw = torch.empty((num_rows, C), dtype=grad.dtype, device=grad.device)
+    with _on(grad.device):
+        ws = ops.workspace(embedding_grad_workspace_bytes(index.numel(), num_rows, C), grad.device)
+        launch_embedding_grad(index, grad, dw, ws, scale)
+    return dw
+
+
+class _EmbeddingGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, index, num_rows, scale):
+        ctx.save_for_backward(index)
+        ctx.rows, ctx.scale = num_rows, scale
+        return _embedding_grad(grad, index, num_rows, scale)
+
+    @staticmethod
+    def backward(ctx, dw):
+        index, = ctx.saved_tensors   # (an index outside the table took no part)
+        return embedding(index, dw, ctx.scale), None, None, None
+
+
 def embedding_grad(grad: torch.Tensor, index: torch.Tensor, num_rows: int, scale: float = 1.0) -> torch.Tensor:
     """The gradient of :func:`embedding` in its table, [num_rows, C] in grad's type: row v is
     ``scale`` times the sum of the rows of ``grad`` [*index.shape, C] whose index is v, zeros where
     there is none.  The sum of atoms by their token is the same operator.
 
-    fp32 sums, rounded once, whose order depends on the indexes alone: equal calls give equal bits."""
-    dev = _device("embedding_grad", grad, index)
+    fp32 sums, rounded once, whose order depends on the indexes alone: equal calls give equal bits.
+    Differentiable in ``grad`` (its gradient is the lookup)."""
+    _device("embedding_grad", grad, index)
     if grad.dim() < 1 or grad.shape[:-1] != index.shape:
         raise ValueError(f"embedding_grad expects grad [*index.shape, C], got {tuple(grad.shape)} for index "
                          f"{tuple(index.shape)}")
@@ -152,13 +367,10 @@ def embedding_grad(grad: torch.Tensor, index: torch.Tensor, num_rows: int, scale
     num_rows = operator.index(num_rows)
     if num_rows < 0:
         raise ValueError(f"embedding_grad: num_rows is negative ({num_rows})")
-    index, grad = _index("embedding_grad", index), _dense(grad)
-    C = grad.shape[-1]
-    dw = torch.empty((num_rows, C), dtype=grad.dtype, device=dev)
-    with _on(dev):
-        ws = ops.workspace(embedding_grad_workspace_bytes(index.numel(), num_rows, C), dev)
-        launch_embedding_grad(index, grad, dw, ws, scale)
-    return dw
+    index = _index("embedding_grad", index)
+    if _wants_grad(grad):
+        return _EmbeddingGrad.apply(grad, index, num_rows, float(scale))
+    return _embedding_grad(grad, index, num_rows, float(scale))
 
 
 # --------------------------------------------------------------------------------------
@@ -199,12 +411,11 @@ class _DropoutAdd(torch.autograd.Function):
         return _dropout_add(x, residual, p, seed, offset, shared)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         p, seed, offset, shared = ctx.args
         if seed is None:
             seed, = ctx.saved_tensors
-        dx = _dropout_add(grad, None, p, seed, offset, shared) if ctx.needs_input_grad[0] else None
+        dx = dropout_add(grad, None, p, seed, offset, shared) if ctx.needs_input_grad[0] else None
         return dx, grad if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
@@ -223,7 +434,7 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, see
     2^64) or an int64 device tensor of one element, read when the kernel runs: a captured graph draws
     new masks when that tensor is written between replays.  Dropped elements are not used, so a NaN
     among them does not spread; p = 1 drops all."""
-    dev = _device("dropout_add", x, residual, seed if isinstance(seed, torch.Tensor) else None)
+    _device("dropout_add", x, residual, seed if isinstance(seed, torch.Tensor) else None)
     _code("dropout_add", x)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"dropout_add: residual {tuple(residual.shape)} {residual.dtype} is not like x "
