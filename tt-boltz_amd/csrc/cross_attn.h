@@ -26,7 +26,8 @@ struct XaParams {
   // backward
   const void* dout;              // [B][Lq][H][D]
   float* delta;                  // [B][H][Lq]
-  const uint32_t* amax;          // [B][Hk][2]: bits of max |dout_i|^2 and max |v_j|^2 (fp16)
+  const float* amax;             // [B][Hk][chunks][2]: largest |dout_i|^2 and |v_j|^2 of a chunk (fp16)
+  int chunks;                    // <= 64
   float* ds;                     // [B][H][Lq][Lk] gradient of the logits, or null
   void *dq, *dk, *dv;            // contiguous
 };
@@ -36,15 +37,15 @@ constexpr int XA_KEYS = 128;                  // keys per workgroup of the dk, d
 constexpr int xa_rt(int dp, bool fp32) { return dp == 128 || fp32 ? 32 : 64; }   // its rows per tile
 
 int pf_xa_fwd_fp32(const XaParams& p, hipStream_t st);
-int pf_xa_delta_fp32(const XaParams& p, float* delta, uint32_t* amax, hipStream_t st);
+int pf_xa_delta_fp32(const XaParams& p, float* amax, hipStream_t st);
 int pf_xa_dq_fp32(const XaParams& p, hipStream_t st);
 int pf_xa_dkv_fp32(const XaParams& p, hipStream_t st);
 int pf_xa_fwd_fp16(const XaParams& p, hipStream_t st);
-int pf_xa_delta_fp16(const XaParams& p, float* delta, uint32_t* amax, hipStream_t st);
+int pf_xa_delta_fp16(const XaParams& p, float* amax, hipStream_t st);
 int pf_xa_dq_fp16(const XaParams& p, hipStream_t st);
 int pf_xa_dkv_fp16(const XaParams& p, hipStream_t st);
 int pf_xa_fwd_bf16(const XaParams& p, hipStream_t st);
-int pf_xa_delta_bf16(const XaParams& p, float* delta, uint32_t* amax, hipStream_t st);
+int pf_xa_delta_bf16(const XaParams& p, float* amax, hipStream_t st);
 int pf_xa_dq_bf16(const XaParams& p, hipStream_t st);
 int pf_xa_dkv_bf16(const XaParams& p, hipStream_t st);
 int pf_xa_exact_delta_fp16(const XaParams& p, hipStream_t st);

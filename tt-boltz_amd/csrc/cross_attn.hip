@@ -4,8 +4,8 @@
 
 namespace {
 
-// Workgroups wanted: two for each of 256 CUs and the next two ready behind them.
-constexpr long WANT = 1024;
+// Workgroups wanted: two for each of 256 CUs.
+constexpr long WANT = 512;
 
 struct Split { int splits, per; };
 
@@ -63,6 +63,8 @@ XaParams params_of(const pf_cross_attn_args* a) {
   if (a->stats) p.st_m = a->stats, p.st_l = a->stats + (long)a->B * a->H * a->Lq;
   p.few = p.rows <= 32;
   p.splits = p.per = 1;
+  const int longest = p.rows > p.Lk ? p.rows : p.Lk;
+  p.chunks = longest > 64 * 128 ? 64 : (longest + 127) / 128;
   return p;
 }
 
@@ -87,7 +89,7 @@ BwdLayout bwd_layout(const pf_cross_attn_args* a, const XaParams& p) {
   BwdLayout l;
   l.delta = 0;
   l.amax = up256((long)p.B * p.H * p.Lq * 4);
-  l.ds = l.amax + up256((long)p.B * p.Hk * 8);
+  l.ds = l.amax + up256((long)p.B * p.Hk * p.chunks * 8);
   const bool own = a->dbias_B > 0 && !(a->bias_dtype == PF_FP32 && a->dbias_B == a->B && a->dbias_H == a->H);
   l.part = l.ds + (own ? up256((long)p.B * p.H * p.Lq * p.Lk * 4) : 0);
   const Split ks = key_split(p), rs = row_split(p, a->dtype);
@@ -100,15 +102,9 @@ BwdLayout bwd_layout(const pf_cross_attn_args* a, const XaParams& p) {
 bool grid_fits(const XaParams& p) {   // a launch holds fewer than 2^32 threads
   const long rt = ((long)p.rows + 31) / 32, kt = ((long)p.Lk + XA_KEYS - 1) / XA_KEYS;
   const long most = (rt > kt ? rt : kt) * p.B;
-  if (most >= (1l << 24) || most * p.Hk >= (1l << 24)) return false;
+  if (most >= (1l << 24) || most * p.Hk >= (1l << 24) || (long)p.B * p.Hk > 65535) return false;
   const long q = (long)p.B * p.Lq * p.H, k = (long)p.B * p.Lk * p.Hk;   // rows: 8 threads each, or one for 4 channels
   return q + k < (1l << 29) && q * p.D < (1l << 34) && k * p.D < (1l << 34);
-}
-
-// Whole-number maxima from 0 (no memset: the call may be captured into a graph).
-__global__ void xa_clear_kernel(uint32_t* a, long n) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) a[i] = 0;
 }
 
 // dbias[bb, hh, e] = sum of ds[b, h, e] over the dimensions of size 1, e < Lq Lk: lanes on neighbouring
@@ -196,21 +192,17 @@ extern "C" int pf_cross_attn_bwd(const pf_cross_attn_args* a) {
   hipStream_t st = (hipStream_t)a->stream;
   char* ws = (char*)a->workspace;
   float* delta = (float*)(ws + l.delta);
-  uint32_t* amax = (uint32_t*)(ws + l.amax);
-  p.dout = a->dout, p.delta = delta, p.amax = amax, p.part = (float*)(ws + l.part);
+  float* amax = (float*)(ws + l.amax);
+  p.dout = a->dout, p.amax = amax, p.part = (float*)(ws + l.part);
   p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
   const int t = a->dtype;
-  if (t == PF_FP16) {
-    const long n = 2l * a->B * a->Hk;
-    xa_clear_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(amax, n);
-    PF_CHECK_LAUNCH("xa_clear_kernel");
-  }
-  float* const by_o = exact ? nullptr : delta;
-  if (int rc = t == PF_FP32   ? pf_xa_delta_fp32(p, by_o, amax, st)
-               : t == PF_FP16 ? pf_xa_delta_fp16(p, by_o, amax, st)
+  p.delta = exact ? nullptr : delta;
+  if (int rc = t == PF_FP32   ? pf_xa_delta_fp32(p, amax, st)
+               : t == PF_FP16 ? pf_xa_delta_fp16(p, amax, st)
                : exact        ? PF_OK
-                              : pf_xa_delta_bf16(p, by_o, amax, st))
+                              : pf_xa_delta_bf16(p, amax, st))
     return rc;
+  p.delta = delta;
   if (exact) {
     const Split s = key_split(p);
     XaParams d = p;

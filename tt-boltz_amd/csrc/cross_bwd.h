@@ -17,8 +17,12 @@ constexpr bool SCALED = __is_same(T, half_t);
 
 // power of two that brings 2 |do| |v| to (2^13, 2^14] (1 where the bound is 0 or not finite)
 PF_DEV float ds_scale(const XaParams& p, int b, int hk) {
-  const uint32_t* a = p.amax + 2 * ((long)b * p.Hk + hk);
-  const float bound = 2.f * __fsqrt_rn(__uint_as_float(a[0])) * __fsqrt_rn(__uint_as_float(a[1]));
+  const float* a = p.amax + ((long)b * p.Hk + hk) * p.chunks * 2;
+  const int lane = threadIdx.x & 63;
+  float g = lane < p.chunks ? a[2 * lane] : 0.f, v = lane < p.chunks ? a[2 * lane + 1] : 0.f;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) g = fmaxf(g, __shfl_xor(g, o)), v = fmaxf(v, __shfl_xor(v, o));
+  const float bound = 2.f * __fsqrt_rn(g) * __fsqrt_rn(v);
   if (!(bound > 0.f) || !(bound < 3.0e38f)) return 1.f;
   int e;
   (void)frexpf(bound, &e);
@@ -26,51 +30,64 @@ PF_DEV float ds_scale(const XaParams& p, int b, int hk) {
 }
 
 // ------------------------------------------------------------------------------ delta
-// delta_i = do_i . o_i in fp32 from the unrounded o (delta null: not wanted), 8 lanes a row.  fp16: also the largest |do_i|^2
-// and |v_j|^2 of a key head (maxima of non-negative floats as whole numbers: any order gives the same).
+// delta_i = do_i . o_i in fp32 from the unrounded o (p.delta null: not wanted), 8 lanes a row; fp16:
+// also the largest |do_i|^2 and |v_j|^2 of the workgroup's part of a key head (ds_scale joins the parts).
+// blockIdx.x: the part (at most 64), blockIdx.y: batch element and key head.
 template <typename T>
-__global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __restrict__ delta, uint32_t* amax) {
-  const long rows = (long)p.B * p.Lq * p.H, keys = SCALED<T> ? (long)p.B * p.Lk * p.Hk : 0;
+__global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __restrict__ amax) {
+  __shared__ float top[2][4];
   const int sub = threadIdx.x & 7;
+  const long b = blockIdx.y / p.Hk;
+  const int hk = blockIdx.y % p.Hk;
   const float* o32 = p.o32 ? p.o32 : (const float*)p.o;
-  const long row = ((long)blockIdx.x * 256 + threadIdx.x) >> 3;
-  float dot = 0.f, sq = 0.f;
-  if (row < rows) {
-    for (int d = 4 * sub; d < p.D; d += 32)
+  float g_top = 0.f, v_top = 0.f;
+  for (int r = blockIdx.x * 32 + (threadIdx.x >> 3); r < p.rows; r += 32 * gridDim.x) {
+    const int i = r / p.G, head = hk * p.G + r - i * p.G;
+    const long at = ((b * p.Lq + i) * p.H + head) * p.D;
+    float dot = 0.f, sq = 0.f;
+    for (int d = 4 * sub; d < p.D; d += 32) {
+      typedef T quad __attribute__((ext_vector_type(4)));
+      const quad g4 = *reinterpret_cast<const quad*>((const T*)p.dout + at + d);
+      const f32x4 o4 = p.delta ? *reinterpret_cast<const f32x4*>(o32 + at + d) : (f32x4)(0.f);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float g = (float)((const T*)p.dout)[row * p.D + d + e];
-        if (delta) dot += g * o32[row * p.D + d + e];
-        sq += g * g;
+        dot = fmaf((float)g4[e], o4[e], dot);
+        sq = fmaf((float)g4[e], (float)g4[e], sq);
       }
-  } else if (row < rows + keys) {
-    const long j = row - rows, bl = j / p.Hk, b = bl / p.Lk;
-    const int hk = (int)(j - bl * p.Hk), key = (int)(bl - b * p.Lk);
-    const bool seen = key < length_of(p, (int)b) && (!p.mask || p.mask[b * p.mb + key]);
-    const T* v = (const T*)p.v + b * p.vb + key * p.vl + hk * p.vh;
-    if (seen)
-      for (int d = 4 * sub; d < p.D; d += 32)
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float g = (float)v[d + e];
-          sq += g * g;
+    for (int o = 1; o < 8; o <<= 1) {
+      dot += __shfl_xor(dot, o);
+      sq += __shfl_xor(sq, o);
+    }
+    if (sub == 0 && p.delta) p.delta[(b * p.H + head) * p.Lq + i] = dot;
+    g_top = fmaxf(g_top, sq);
+  }
+  if constexpr (SCALED<T>) {
+    const int len = length_of(p, (int)b);
+    for (int key = blockIdx.x * 32 + (threadIdx.x >> 3); key < len; key += 32 * gridDim.x) {
+      float sq = 0.f;
+      if (!p.mask || p.mask[b * p.mb + key]) {
+        const T* v = (const T*)p.v + b * p.vb + key * p.vl + hk * p.vh;
+        for (int d = 4 * sub; d < p.D; d += 32) {
+          typedef T quad __attribute__((ext_vector_type(4)));
+          const quad v4 = *reinterpret_cast<const quad*>(v + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sq = fmaf((float)v4[e], (float)v4[e], sq);
         }
-  }
+      }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    dot += __shfl_xor(dot, o);
-    sq += __shfl_xor(sq, o);
-  }
-  if (sub != 0) return;
-  if (row < rows) {
-    const long bl = row / p.H;
-    const int head = (int)(row - bl * p.H);
-    const long b = bl / p.Lq, i = bl - b * p.Lq;
-    if (delta) delta[(b * p.H + head) * p.Lq + i] = dot;
-    if constexpr (SCALED<T>) atomicMax(amax + 2 * (b * p.Hk + head / p.G), __float_as_uint(sq));
-  } else if (row < rows + keys) {
-    const long j = row - rows, bl = j / p.Hk;
-    atomicMax(amax + 2 * (bl / p.Lk * p.Hk + (j - bl * p.Hk)) + 1, __float_as_uint(sq));
+      for (int o = 1; o < 8; o <<= 1) sq += __shfl_xor(sq, o);
+      v_top = fmaxf(v_top, sq);
+    }
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) g_top = fmaxf(g_top, __shfl_xor(g_top, o)), v_top = fmaxf(v_top, __shfl_xor(v_top, o));
+    if ((threadIdx.x & 63) == 0) top[0][threadIdx.x >> 6] = g_top, top[1][threadIdx.x >> 6] = v_top;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const float* t = top[threadIdx.x];
+      amax[((long)blockIdx.y * gridDim.x + blockIdx.x) * 2 + threadIdx.x] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+    }
   }
 }
 
@@ -79,13 +96,13 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
 // be made of.  A bias's gradient is dS itself, in fp32 as a rule, and do . o is not good enough for it:
 // 16-bit types round P in o's product (2^-9 or 2^-12 of delta, against 2^-22 here).
 template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
-__global__ __launch_bounds__(256) void xa_dq_kernel(XaParams p) {
+__global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP);
   extern __shared__ __align__(16) char smem[];
-  T* const ks = reinterpret_cast<T*>(smem);
-  T* const vs = ks + KT * KS;
+  constexpr int BUF = 2 * KT * KS, NBUF = buffers<T, FEW>();
+  T* const ks0 = reinterpret_cast<T*>(smem);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
   constexpr int ROWS = FEW ? 32 : 128;
   const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
@@ -104,14 +121,8 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaParams p) {
   const float sf = SCALED<T> && !DELTA ? ds_scale(p, b, hk) : 1.f;
   float sum = 0.f;   // DELTA: this lane's half of the keys
   const char* bias = nullptr;
-  bool bias_vec = false;
-  if constexpr (BIAS) {
-    const long at = b * p.bb + head * p.bh + i * p.bq;
-    bias = (const char*)p.bias + at * (p.bias_f32 ? 4 : (long)sizeof(T));
-    bias_vec = p.bk == 1 && ((p.bb | p.bh | p.bq) & 3) == 0 && ((uintptr_t)p.bias & 15) == 0;
-  }
+  if constexpr (BIAS) bias = bias_row<T>(p, b, head, i);
   float* const ds = !DELTA && p.ds && row_ok ? p.ds + stat * p.Lk : nullptr;
-  const bool ds_vec = (p.Lk & 3) == 0;
   const int len = length_of(p, b);
   // the logits' gradient has zeros at hidden keys, so its writer goes on to the end
   const int t0 = blk.z * p.per, t1 = min(t0 + p.per, ((!DELTA && p.ds ? p.Lk : len) + KT - 1) / KT);
@@ -121,12 +132,8 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaParams p) {
 
   Stage<T, DP, KT> sk, sv;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    auto seen = [&](int row) __attribute__((always_inline)) {
-      const int key = t * KT + row;
-      return key < len && (!mask || mask[key]);
-    };
-    sk.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? kb + (long)(t * KT + row) * p.kl : nullptr; });
-    sv.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? vb + (long)(t * KT + row) * p.vl : nullptr; });
+    load_keys<T, DP, KT>(sk, kb, p.kl, p.D, t, len, mask);
+    load_keys<T, DP, KT>(sv, vb, p.vl, p.D, t, len, mask);
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;
@@ -134,50 +141,74 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaParams p) {
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
 
-  if (t0 < t1) load_tile(t0);
+  if (t0 < t1) {
+    load_tile(t0);
+    sk.store(ks0, KS);
+    sv.store(ks0 + KT * KS, KS);
+  }
+  __syncthreads();
   for (int t = t0; t < t1; ++t) {
-    sk.store(ks, KS);
-    sv.store(vs, KS);
-    __syncthreads();
+    const T* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    const T* const vs = ks + KT * KS;
     if (t + 1 < t1) load_tile(t + 1);
-    const int key_l = t * KT + sub0 + (FEW ? n : lane);
-    const uint64_t word = __ballot(key_l < len && (!mask || mask[key_l]));
+    uint64_t word = ~0ull;
+    if (mask || (t + 1) * KT > len) {
+      const int key_l = t * KT + sub0 + (FEW ? n : lane);
+      word = __ballot(key_l < len && (!mask || mask[key_l]));
+    }
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
       const uint32_t word_u = (uint32_t)(word >> (FEW ? 0 : 32 * u));
       if (!word_u && (DELTA || !p.ds)) continue;
+      const int key0 = t * KT + sub0 + 32 * u + 4 * h;
+      float bs[4][4];
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int run = 0; run < 4; ++run) load_bias<T>(p, bias, key0 + 8 * run, row_ok, bs[run]);
+      }
       const int at = (sub0 + 32 * u + n) * KS + M::E * h;
       const f32x16 s = inner<T, DP>(ks + at, q, zero16());
-      f32x16 dp;
+      f32x16 y;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) dp[k] = -delta;
-      dp = inner<T, DP>(vs + at, g, dp);
-      const uint32_t w = word_u >> (4 * h);
+      for (int k = 0; k < 16; ++k) y[k] = -delta;
+      y = inner<T, DP>(vs + at, g, y);
 #pragma unroll
-      for (int run = 0; run < 4; ++run) {
-        const int key = t * KT + sub0 + 32 * u + 8 * run + 4 * h;
-        float bs[4], y[4];
-        if constexpr (BIAS) load_bias<T>(p, bias, key, row_ok, bias_vec, bs);
+      for (int k = 0; k < 16; ++k)
+        y[k] *= exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[k >> 2][k & 3]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
+      if (word_u != 0xffffffffu) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 4 * run + e;
-          const float pr = exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[e]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
-          const bool seen = (w >> acc_row(k, 0)) & 1;
-          y[e] = seen ? pr * dp[k] : 0.f;
-          if constexpr (DELTA) sum += y[e];
-          dp[k] = SCALED<T> ? y[e] * sf : y[e];
-        }
-        if (ds) {
-          if (ds_vec && key < p.Lk) {
-            store4<float>(ds + key, y);
+        for (int k = 0; k < 16; ++k) y[k] = (word_u >> (4 * h) >> acc_row(k, 0)) & 1 ? y[k] : 0.f;
+      }
+      if constexpr (DELTA) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += y[k];
+        continue;
+      }
+      if (ds) {
+#pragma unroll
+        for (int run = 0; run < 4; ++run) {
+          const int key = key0 + 8 * run;
+          if (key + 3 < p.Lk) {
+            const typename Any4<float>::type v = {y[4 * run], y[4 * run + 1], y[4 * run + 2], y[4 * run + 3]};
+            *reinterpret_cast<typename Any4<float>::type*>(ds + key) = v;
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (key + e < p.Lk) ds[key + e] = y[e];
+              if (key + e < p.Lk) ds[key + e] = y[4 * run + e];
           }
         }
       }
-      if (!DELTA && word_u) M::template outer<DT>(ks + (sub0 + 32 * u) * KS, KS, lane, dp, dq);
+      if constexpr (SCALED<T>) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] *= sf;
+      }
+      if (word_u) M::template outer<DT>(ks + (sub0 + 32 * u) * KS, KS, lane, M::pack(y), dq);
+    }
+    if constexpr (NBUF == 1) __syncthreads();
+    if (t + 1 < t1) {
+      T* const to = ks0 + (NBUF == 2 ? (t + 1 - t0) % 2 * BUF : 0);
+      sk.store(to, KS);
+      sv.store(to + KT * KS, KS);
     }
     __syncthreads();
   }
@@ -242,7 +273,7 @@ __global__ __launch_bounds__(256) void xa_dq_kernel(XaParams p) {
 
 // ------------------------------------------------------------------------------ dk, dv
 template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256) void xa_dkv_kernel(XaParams p) {
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xa_dkv_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::row_stride(DP);
   extern __shared__ __align__(16) char smem[];
@@ -270,13 +301,13 @@ __global__ __launch_bounds__(256) void xa_dkv_kernel(XaParams p) {
   float stat = 0.f;   // threads 0 .. 3 RT: one value of the tile's statistics
   const int sw = threadIdx.x / RT, sr = threadIdx.x % RT;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    sq.load(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
+    sq.gather(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
       const int r = t * RT + row;
       if (r >= p.rows) return nullptr;
       const int i = r / p.G, head = hk * p.G + r - i * p.G;
       return (const T*)p.q + b * p.qb + i * p.ql + head * p.qh;
     });
-    sg.load(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
+    sg.gather(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
       const int r = t * RT + row;
       if (r >= p.rows) return nullptr;
       const int i = r / p.G, head = hk * p.G + r - i * p.G;
@@ -340,8 +371,8 @@ __global__ __launch_bounds__(256) void xa_dkv_kernel(XaParams p) {
             dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
           }
         }
-        M::template outer<DT>(gs + 32 * u * S, S, lane, pr, dv);
-        M::template outer<DT>(qs + 32 * u * S, S, lane, dp, dk);
+        M::template outer<DT>(gs + 32 * u * S, S, lane, M::pack(pr), dv);
+        M::template outer<DT>(qs + 32 * u * S, S, lane, M::pack(dp), dk);
       }
     }
     __syncthreads();
@@ -372,10 +403,13 @@ __global__ __launch_bounds__(256) void xa_dkv_kernel(XaParams p) {
     }
 }
 
-// out = the sum over `splits` of part[z * step + e], four elements a thread
+// out = the sum over `splits` of part[z * step + e], e < n, four elements a thread; blockIdx.y = 1: the
+// second result, its parts n behind the first's
 template <typename T>
-__global__ __launch_bounds__(256) void xa_sum_kernel(const float* __restrict__ part, long step, int splits, T* __restrict__ out,
-                                                     long n) {
+__global__ __launch_bounds__(256) void xa_sum_kernel(const float* __restrict__ part, long step, int splits, T* __restrict__ out0,
+                                                     T* __restrict__ out1, long n) {
+  T* const out = blockIdx.y ? out1 : out0;
+  part += blockIdx.y * n;
   const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (e >= n) return;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
@@ -396,8 +430,8 @@ __global__ __launch_bounds__(256) void xa_sum_kernel(const float* __restrict__ p
 }
 
 template <typename T>
-int sum_launch(const float* part, long step, int splits, void* out, long n, hipStream_t st) {
-  xa_sum_kernel<T><<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(part, step, splits, (T*)out, n);
+int sum_launch(const float* part, long step, int splits, void* out0, void* out1, long n, hipStream_t st) {
+  xa_sum_kernel<T><<<dim3((unsigned)((n + 1023) / 1024), out1 ? 2 : 1), 256, 0, st>>>(part, step, splits, (T*)out0, (T*)out1, n);
   PF_CHECK_LAUNCH("xa_sum_kernel");
   return PF_OK;
 }
@@ -405,7 +439,7 @@ int sum_launch(const float* part, long step, int splits, void* out, long n, hipS
 template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
 int dq_launch(const XaParams& p, hipStream_t st) {
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
-  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * sizeof(T), join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0;
+  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * sizeof(T) * buffers<T, FEW>(), join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0;
   const size_t lds = tiles > join ? tiles : join;
   if (int rc = pf_reserve_lds((const void*)xa_dq_kernel<T, DP, BIAS, FEW, DELTA>, lds, "xa_dq_kernel")) return rc;
   const int rt = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
@@ -413,8 +447,8 @@ int dq_launch(const XaParams& p, hipStream_t st) {
   PF_CHECK_LAUNCH("xa_dq_kernel");
   if (p.splits == 1) return PF_OK;
   const long rows = (long)p.B * p.Lq * p.H;
-  return DELTA ? sum_launch<float>(p.part, rows, p.splits, (float*)p.delta, rows, st)
-               : sum_launch<T>(p.part, rows * p.D, p.splits, p.dq, rows * p.D, st);
+  return DELTA ? sum_launch<float>(p.part, rows, p.splits, p.delta, nullptr, rows, st)
+               : sum_launch<T>(p.part, rows * p.D, p.splits, p.dq, nullptr, rows * p.D, st);
 }
 
 template <typename T, int DP>
@@ -449,8 +483,7 @@ int dkv_launch(const XaParams& p, hipStream_t st) {
   PF_CHECK_LAUNCH("xa_dkv_kernel");
   if (p.splits == 1) return PF_OK;
   const long n = (long)p.B * p.Lk * p.Hk * p.D;
-  if (int rc = sum_launch<T>(p.part, 2 * n, p.splits, p.dk, n, st)) return rc;
-  return sum_launch<T>(p.part + n, 2 * n, p.splits, p.dv, n, st);
+  return sum_launch<T>(p.part, 2 * n, p.splits, p.dk, p.dv, n, st);
 }
 
 template <typename T, int DP>
@@ -464,9 +497,8 @@ int dkv_type(const XaParams& p, hipStream_t st) {
 }
 
 template <typename T>
-int delta_type(const XaParams& p, float* delta, uint32_t* amax, hipStream_t st) {
-  const long rows = (long)p.B * p.Lq * p.H + (SCALED<T> ? (long)p.B * p.Lk * p.Hk : 0);
-  xa_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(p, delta, amax);
+int delta_type(const XaParams& p, float* amax, hipStream_t st) {
+  xa_delta_kernel<T><<<dim3((unsigned)p.chunks, (unsigned)(p.B * p.Hk)), 256, 0, st>>>(p, amax);
   PF_CHECK_LAUNCH("xa_delta_kernel");
   return PF_OK;
 }

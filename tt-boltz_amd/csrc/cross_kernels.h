@@ -48,25 +48,44 @@ struct Mma {
     if constexpr (__is_same(T, half_t)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // acc[dt] += X^T p over 32 rows of the LDS tile X (row stride `st`): p is an accumulator, and X's
-  // rows are taken in its order.  A transposing read hands lane i of 16 the column i of a 4 x 16 block
-  // whose 8-byte pieces the lanes point at.
+  // an accumulator as the right operand of a product over its 32 rows
+  struct Packed { frag_t f[2]; };
+  static PF_DEV Packed pack(const f32x16& p) {
+    Packed b;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) b.f[s][t] = (T)p[8 * s + t];
+    return b;
+  }
+  // c + the sum of this lane's 16 values as they were rounded
+  static PF_DEV float sum(const Packed& b, float c) {
+    typedef T pair_t __attribute__((ext_vector_type(2)));
+    const pair_t one = {(T)1.f, (T)1.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) {
+        const pair_t v = {b.f[s][t], b.f[s][t + 1]};
+        if constexpr (__is_same(T, half_t)) c = __builtin_amdgcn_fdot2(v, one, c, false);
+        else c = __builtin_amdgcn_fdot2_f32_bf16(v, one, c, false);
+      }
+    return c;
+  }
+  // acc[dt] += X^T P over 32 rows of the LDS tile X (row stride `st`), taken in P's order.  A transposing
+  // read hands lane i of 16 the column i of a 4 x 16 block whose 8-byte pieces the lanes point at.
   template <int DT>
-  static PF_DEV void outer(const T* x, int st, int lane, const f32x16& p, f32x16 (&acc)[DT]) {
+  static PF_DEV void outer(const T* x, int st, int lane, const Packed& p, f32x16 (&acc)[DT]) {
     const int h = lane >> 5, i = lane & 15, c16 = (lane >> 4) & 1;
     const T* at = x + (4 * h + (i >> 2)) * st + 16 * c16 + 4 * (i & 3);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      frag_t b;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) b[t] = (T)p[8 * s + t];
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const quad_t lo = tr_read(at + (16 * s) * st + 32 * dt), hi = tr_read(at + (16 * s + 8) * st + 32 * dt);
         const frag_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[dt] = mma(a, b, acc[dt]);
+        acc[dt] = mma(a, p.f[s], acc[dt]);
       }
-    }
   }
   static PF_DEV quad_t tr_read(const T* p) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -84,6 +103,13 @@ struct Mma<float> {
   static PF_DEV f32x16 mma(const frag_t& a, const frag_t& b, f32x16 c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  typedef f32x16 Packed;
+  static PF_DEV Packed pack(const f32x16& p) { return p; }
+  static PF_DEV float sum(const Packed& b, float c) {
+#pragma unroll
+    for (int t = 0; t < 16; ++t) c += b[t];
     return c;
   }
   template <int DT>
@@ -122,35 +148,72 @@ PF_DEV f32x16 inner(const T* a, const Frag<T, DP>& b, f32x16 c) {
   return c;
 }
 
-// A tile of ROWS rows x DP channels on its way from global memory to LDS: 16-byte pieces in registers.
+// A tile of ROWS rows x DP channels on its way from global memory to LDS: 16-byte pieces in registers,
+// a thread's pieces in one column of pieces, 256 / PER rows apart.
 template <typename T, int DP, int ROWS>
 struct Stage {
   typedef typename Vec16<T>::type vec_t;
-  static constexpr int N = Vec16<T>::N, PER = DP / N, CH = ROWS * PER / 256;
-  static_assert(ROWS * PER % 256 == 0, "whole pieces per thread");
+  static constexpr int N = Vec16<T>::N, PER = DP / N, CH = ROWS * PER / 256, STEP = 256 / PER;
+  static_assert(ROWS * PER % 256 == 0 && 256 % PER == 0, "whole pieces per thread");
   vec_t v[CH];
-  // row(r): the row's address, or null (zeros)
+  static PF_DEV int row(int j) { return (int)threadIdx.x / PER + j * STEP; }
+  static PF_DEV int chan() { return (int)threadIdx.x % PER * N; }
+  // p: row 0 of the tile, rows `stride` apart; all rows are there
+  PF_DEV void load(const T* p, long stride, int D) {
+    const vec_t z = {};
+    if (chan() < D) {
+      p += row(0) * stride + chan();
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = *reinterpret_cast<const vec_t*>(p + j * STEP * stride);
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = z;
+    }
+  }
+  // rows with bit row(j) of `rows(j)` only, zeros for the others
   template <typename F>
-  PF_DEV void load(int D, F row) {
+  PF_DEV void load_some(const T* p, long stride, int D, F there) {
+    p += row(0) * stride + chan();
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      const int c = threadIdx.x + 256 * j, r = c / PER, d = (c % PER) * N;
-      const T* p = row(r);
-      vec_t z = {};
-      v[j] = p && d < D ? *reinterpret_cast<const vec_t*>(p + d) : z;
+      const vec_t z = {};
+      v[j] = chan() < D && there(row(j)) ? *reinterpret_cast<const vec_t*>(p + j * STEP * stride) : z;
+    }
+  }
+  // row(r): its address, or null (zeros)
+  template <typename F>
+  PF_DEV void gather(int D, F at) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const T* p = at(row(j));
+      const vec_t z = {};
+      v[j] = p && chan() < D ? *reinterpret_cast<const vec_t*>(p + chan()) : z;
     }
   }
   PF_DEV void store(T* lds, int stride) const {
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int c = threadIdx.x + 256 * j, r = c / PER, d = (c % PER) * N;
-      *reinterpret_cast<vec_t*>(lds + r * stride + d) = v[j];
-    }
+    for (int j = 0; j < CH; ++j) *reinterpret_cast<vec_t*>(lds + row(j) * stride + chan()) = v[j];
   }
 };
 
-// Consecutive workgroups of one (batch, key head) on one XCD: its keys and values stay in that L2.
-PF_DEV int xcd_remap(int w, int total) { return total % 8 ? w : (w % 8) * (total / 8) + w / 8; }
+// Key tile t of one key head: rows of hidden keys are zeros (what stands there, NaN say, takes no part).
+template <typename T, int DP, int KT>
+PF_DEV void load_keys(Stage<T, DP, KT>& s, const T* base, long stride, int D, int t, int len, const uint8_t* mask) {
+  const T* p = base + (long)t * KT * stride;
+  if (!mask && (t + 1) * KT <= len) s.load(p, stride, D);
+  else
+    s.load_some(p, stride, D, [&](int row) __attribute__((always_inline)) {
+      const int key = t * KT + row;
+      return key < len && (!mask || mask[key]);
+    });
+}
+
+// Workgroup w runs on XCD w % 8: neighbouring ids go to one XCD, so the workgroups of a (batch, key head)
+// share its keys and values in one L2.
+PF_DEV int xcd_remap(int w, int total) {
+  const int x = w % 8, q = total / 8, rem = total % 8;
+  return x * q + min(x, rem) + w / 8;
+}
 
 struct Block { int rt, z, b, hk; };
 PF_DEV Block block_of(const XaParams& p, int tiles) {
@@ -161,29 +224,34 @@ PF_DEV Block block_of(const XaParams& p, int tiles) {
 
 PF_DEV int length_of(const XaParams& p, int b) { return p.lens ? max(0, min(p.Lk, p.lens[b])) : p.Lk; }
 
-// bias[row, key .. key + 3] of a lane's query (0 outside the tensor)
+// 4 elements that need not begin on a multiple of their size together
 template <typename T>
-PF_DEV void load_bias(const XaParams& p, const char* row, int key, bool ok, bool vec, float (&x)[4]) {
+struct Any4 { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
+
+// bias[row, key .. key + 3] of a lane's query (0 outside the tensor); dense: neighbouring keys adjoin
+template <typename B>
+PF_DEV void load_bias4(const B* a, int key, int Lk, bool dense, long bk, float (&x)[4]) {
+  if (dense && key + 3 < Lk) {
+    const auto v = *reinterpret_cast<const typename Any4<B>::type*>(a + key);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = key + e < Lk ? (float)a[(key + e) * bk] : 0.f;
+  }
+}
+template <typename T>
+PF_DEV void load_bias(const XaParams& p, const char* row, int key, bool ok, float (&x)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = 0.f;
-  if (!ok || key >= p.Lk) return;
-  if (p.bias_f32) {
-    const float* a = reinterpret_cast<const float*>(row);
-    if (vec && key + 3 < p.Lk) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a + key);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (key + e < p.Lk) x[e] = a[(key + e) * p.bk];
-    }
-  } else {
-    const T* a = reinterpret_cast<const T*>(row);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (key + e < p.Lk) x[e] = (float)a[(key + e) * p.bk];
-  }
+  if (!ok) return;
+  if (p.bias_f32) load_bias4(reinterpret_cast<const float*>(row), key, p.Lk, p.bk == 1, p.bk, x);
+  else load_bias4(reinterpret_cast<const T*>(row), key, p.Lk, p.bk == 1, p.bk, x);
+}
+// a lane's row of the bias
+template <typename T>
+PF_DEV const char* bias_row(const XaParams& p, int b, int head, int i) {
+  return (const char*)p.bias + (b * p.bb + head * p.bh + i * p.bq) * (p.bias_f32 ? 4 : (long)sizeof(T));
 }
 
 // c s - m, the exponent of a probability without a bias.  fp32 tensors: the product is rounded before
@@ -214,14 +282,23 @@ PF_DEV void store4(T* p, const float (&x)[4]) {
 // FEW = false: 4 waves x 32 rows, every wave over the tile's 64 keys.  FEW = true (at most 32 rows, and
 // few enough tiles): the waves share a 32-row tile and take 32 of the tile's 128 keys each; their
 // results are joined through LDS.
+// LDS buffers of a tile: two, so that a tile needs one barrier, or one where the tiles are large and more
+// workgroups per CU are worth more (single rows stream keys at memory's rate).
+template <typename T, bool FEW>
+constexpr int buffers() { return FEW || __is_same(T, float) ? 1 : 2; }
+
+// Waves per SIMD that a kernel's registers are kept to: two, where 256 registers hold it.
+template <typename T, int DP, bool FEW>
+constexpr int waves() { return DP == 128 && (FEW || __is_same(T, float)) ? 1 : 2; }
+
 template <typename T, int DP, bool BIAS, bool FEW>
-__global__ __launch_bounds__(256) void xa_fwd_kernel(XaParams p) {
+__global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP), VS = M::col_stride(DP);
   extern __shared__ __align__(16) char smem[];
-  T* const ks = reinterpret_cast<T*>(smem);
-  T* const vs = ks + KT * KS;
+  constexpr int BUF = KT * (KS + VS), NBUF = buffers<T, FEW>();
+  T* const ks0 = reinterpret_cast<T*>(smem);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
   constexpr int ROWS = FEW ? 32 : 128;
   const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
@@ -233,12 +310,7 @@ __global__ __launch_bounds__(256) void xa_fwd_kernel(XaParams p) {
   Frag<T, DP> q;
   q.load((const T*)p.q + b * p.qb + i * p.ql + head * p.qh, p.D, h, row_ok, p.neg);
   const char* bias = nullptr;
-  bool bias_vec = false;
-  if constexpr (BIAS) {
-    const long at = b * p.bb + head * p.bh + i * p.bq;
-    bias = (const char*)p.bias + at * (p.bias_f32 ? 4 : (long)sizeof(T));
-    bias_vec = p.bk == 1 && ((p.bb | p.bh | p.bq) & 3) == 0 && ((uintptr_t)p.bias & 15) == 0;
-  }
+  if constexpr (BIAS) bias = bias_row<T>(p, b, head, i);
   const int len = length_of(p, b);
   const int t0 = blk.z * p.per, t1 = min(t0 + p.per, (len + KT - 1) / KT);
   const uint8_t* mask = p.mask ? p.mask + b * p.mb : nullptr;
@@ -247,54 +319,60 @@ __global__ __launch_bounds__(256) void xa_fwd_kernel(XaParams p) {
 
   Stage<T, DP, KT> sk, sv;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    // a hidden key's rows are zeros: what stands there (NaN, say) takes no part
-    auto seen = [&](int row) __attribute__((always_inline)) {
-      const int key = t * KT + row;
-      return key < len && (!mask || mask[key]);
-    };
-    sk.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? kb + (long)(t * KT + row) * p.kl : nullptr; });
-    sv.load(p.D, [&](int row) __attribute__((always_inline)) { return seen(row) ? vb + (long)(t * KT + row) * p.vl : nullptr; });
+    load_keys<T, DP, KT>(sk, kb, p.kl, p.D, t, len, mask);
+    load_keys<T, DP, KT>(sv, vb, p.vl, p.D, t, len, mask);
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;   // x in units of 1 (bias) or log2
+  // the reference of the exponentials follows the maximum when that has grown by SLACK: p <= 2^8
+  constexpr float SLACK = BIAS ? 5.f : 8.f;
   float m = -INFINITY, l = 0.f;                       // l: this lane's half of the keys
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
 
-  if (t0 < t1) load_tile(t0);
+  if (t0 < t1) {
+    load_tile(t0);
+    sk.store(ks0, KS);
+    sv.store(ks0 + KT * KS, VS);
+  }
+  __syncthreads();
   for (int t = t0; t < t1; ++t) {
-    sk.store(ks, KS);
-    sv.store(vs, VS);
-    __syncthreads();
+    const T* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    const T* const vs = ks + KT * KS;
     if (t + 1 < t1) load_tile(t + 1);
     // the keys of this wave that are seen, bit j: key sub0 + j of the tile
-    const int key_l = t * KT + sub0 + (FEW ? n : lane);
-    const uint64_t word = __ballot(key_l < len && (!mask || mask[key_l]));
+    uint64_t word = ~0ull;
+    if (mask || (t + 1) * KT > len) {
+      const int key_l = t * KT + sub0 + (FEW ? n : lane);
+      word = __ballot(key_l < len && (!mask || mask[key_l]));
+    }
     if (word) {
       float x[NSUB][16];
       float mx = -INFINITY;
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
+        float bs[4][4];
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int run = 0; run < 4; ++run)
+            load_bias<T>(p, bias, t * KT + sub0 + 32 * u + 8 * run + 4 * h, row_ok, bs[run]);
+        }
         const f32x16 s = inner<T, DP>(ks + (sub0 + 32 * u + n) * KS + M::E * h, q, zero16());
 #pragma unroll
-        for (int run = 0; run < 4; ++run) {
-          float bs[4];
-          if constexpr (BIAS) load_bias<T>(p, bias, t * KT + sub0 + 32 * u + 8 * run + 4 * h, row_ok, bias_vec, bs);
+        for (int k = 0; k < 16; ++k) x[u][k] = BIAS ? fmaf(s[k], c, bs[k >> 2][k & 3]) : s[k];
+        const uint32_t w = (uint32_t)(word >> (FEW ? 0 : 32 * u));
+        if (w != 0xffffffffu) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[u][4 * run + e] = BIAS ? fmaf(s[4 * run + e], c, bs[e]) : s[4 * run + e];
-        }
-        const uint32_t w = (uint32_t)(word >> (FEW ? 0 : 32 * u)) >> (4 * h);
-        if ((uint32_t)(word >> (FEW ? 0 : 32 * u)) != 0xffffffffu) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) x[u][k] = (w >> acc_row(k, 0)) & 1 ? x[u][k] : -INFINITY;
+          for (int k = 0; k < 16; ++k) x[u][k] = (w >> (4 * h) >> acc_row(k, 0)) & 1 ? x[u][k] : -INFINITY;
         }
 #pragma unroll
         for (int k = 0; k < 16; ++k) mx = fmaxf(mx, x[u][k]);
       }
       mx = xor32_max(mx);
-      const float m_new = fmaxf(m, BIAS ? mx : mx * c);
-      if (__any(m_new > m)) {
+      if (!BIAS) mx *= c;
+      if (__any(mx > m + SLACK)) {
+        const float m_new = fmaxf(m, mx);
         const float a = m_new > m ? exp2_fast(BIAS ? (m - m_new) * LOG2E : m - m_new) : 1.f;
         l *= a;
 #pragma unroll
@@ -308,12 +386,22 @@ __global__ __launch_bounds__(256) void xa_fwd_kernel(XaParams p) {
       for (int u = 0; u < NSUB; ++u) {
         f32x16 pr;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          pr[k] = exp2_fast(BIAS ? (x[u][k] - mu) * LOG2E : exponent<T>(x[u][k], c, mu));
-          l += pr[k];
+        for (int k = 0; k < 16; ++k) pr[k] = exp2_fast(BIAS ? (x[u][k] - mu) * LOG2E : exponent<T>(x[u][k], c, mu));
+        const typename M::Packed pk = M::pack(pr);
+        if constexpr (BIAS) {   // the bias's gradient wants P, and so the sum, to fp32
+#pragma unroll
+          for (int k = 0; k < 16; ++k) l += pr[k];
+        } else {
+          l = M::sum(pk, l);
         }
-        M::template outer<DT>(vs + (sub0 + 32 * u) * VS, VS, lane, pr, o);
+        M::template outer<DT>(vs + (sub0 + 32 * u) * VS, VS, lane, pk, o);
       }
+    }
+    if constexpr (NBUF == 1) __syncthreads();
+    if (t + 1 < t1) {
+      T* const to = ks0 + (NBUF == 2 ? (t + 1 - t0) % 2 * BUF : 0);
+      sk.store(to, KS);
+      sv.store(to + KT * KS, VS);
     }
     __syncthreads();
   }
@@ -454,7 +542,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaParams p) {
 template <typename T, int DP, bool FEW>
 size_t fwd_lds() {
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
-  const size_t tiles = (size_t)KT * (Mma<T>::row_stride(DP) + Mma<T>::col_stride(DP)) * sizeof(T);
+  const size_t tiles = (size_t)KT * (Mma<T>::row_stride(DP) + Mma<T>::col_stride(DP)) * sizeof(T) * buffers<T, FEW>();
   const size_t join = FEW ? (size_t)4 * 32 * (DP + 4 + 2) * 4 : 0;
   return tiles > join ? tiles : join;
 }
