@@ -23,6 +23,7 @@ struct XaParams {
   float* part;                   // splits > 1: partial results
   int splits, per;               // key tiles (dkv: row tiles) per split
   int few;                       // the waves of a workgroup share a 32-row tile
+  int wide;                      // forward: two 32-row tiles per wave
   // backward
   const void* dout;              // [B][Lq][H][D]
   float* delta;                  // [B][H][Lq]

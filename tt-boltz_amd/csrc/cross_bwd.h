@@ -95,8 +95,14 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
 // DELTA: delta_i = sum_j P_ij (do_i . v_j) instead, of the split's keys, from the fp32 P and dP that dS will
 // be made of.  A bias's gradient is dS itself, in fp32 as a rule, and do . o is not good enough for it:
 // 16-bit types round P in o's product (2^-9 or 2^-12 of delta, against 2^-22 here).
+template <typename T, int DP, bool BIAS, bool FEW>
+constexpr int dq_waves() {
+  if (DP == 128) return FEW || __is_same(T, float) ? 1 : 2;
+  return __is_same(T, float) || DP == 64 ? 2 : BIAS || FEW ? 3 : 4;
+}
+
 template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
-__global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaParams p) {
+__global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP);
@@ -132,14 +138,14 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaPar
 
   Stage<T, DP, KT> sk, sv;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    load_keys<T, DP, KT>(sk, kb, p.kl, p.D, t, len, mask);
-    load_keys<T, DP, KT>(sv, vb, p.vl, p.D, t, len, mask);
+    load_keys(sk, kb, p.kl, p.D, t, len, mask);
+    load_keys(sv, vb, p.vl, p.D, t, len, mask);
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;
-  f32x16 dq[DT];
+  f32x16 dq[1][DT];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
+  for (int dt = 0; dt < DT; ++dt) dq[0][dt] = zero16();
 
   if (t0 < t1) {
     load_tile(t0);
@@ -202,7 +208,10 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaPar
 #pragma unroll
         for (int k = 0; k < 16; ++k) y[k] *= sf;
       }
-      if (word_u) M::template outer<DT>(ks + (sub0 + 32 * u) * KS, KS, lane, M::pack(y), dq);
+      if (word_u) {
+        const typename M::Packed pk[1] = {M::pack(y)};
+        M::template outer<DT, 1>(ks + (sub0 + 32 * u) * KS, KS, lane, pk, dq);
+      }
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) {
@@ -234,7 +243,7 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaPar
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int run = 0; run < 4; ++run) {
-        const f32x4 v = {dq[dt][4 * run], dq[dt][4 * run + 1], dq[dt][4 * run + 2], dq[dt][4 * run + 3]};
+        const f32x4 v = {dq[0][dt][4 * run], dq[0][dt][4 * run + 1], dq[0][dt][4 * run + 2], dq[0][dt][4 * run + 3]};
         *reinterpret_cast<f32x4*>(os + (32 * wid + n) * OS + 32 * dt + 8 * run + 4 * h) = v;
       }
     __syncthreads();
@@ -264,7 +273,7 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaPar
         if (d >= p.D) continue;
         float a[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = dq[dt][4 * run + e] * out_scale;
+        for (int e = 0; e < 4; ++e) a[e] = dq[0][dt][4 * run + e] * out_scale;
         if (p.splits > 1) store4<float>(p.part + ((long)blk.z * p.B * p.Lq * p.H + row_at) * p.D + d, a);
         else store4<T>((T*)p.dq + row_at * p.D + d, a);
       }
@@ -272,14 +281,21 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_dq_kernel(XaPar
 }
 
 // ------------------------------------------------------------------------------ dk, dv
+// 4 waves x 32 keys; a tile is RT consecutive queries of one head, the heads of the key head one after
+// the other.  A wave's values stay in registers; its keys do too where those suffice for two waves per
+// SIMD, else (128 channels) they are read from LDS for each tile.
+template <typename T, int DP>
+constexpr bool keys_in_lds() { return DP == 128 && !__is_same(T, float); }
+
 template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xa_dkv_kernel(XaParams p) {
+__global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void xa_dkv_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::row_stride(DP);
+  constexpr int NBUF = buffers<T, false>(), STATS = 3 * RT * 4 / (int)sizeof(T), BUF = 2 * RT * S + STATS;
+  constexpr bool KLDS = keys_in_lds<T, DP>();
   extern __shared__ __align__(16) char smem[];
-  T* const qs = reinterpret_cast<T*>(smem);
-  T* const gs = qs + RT * S;
-  float* const st = reinterpret_cast<float*>(gs + RT * S);   // [3][RT]: maximum, log2 of the sum, delta
+  T* const buf0 = reinterpret_cast<T*>(smem);   // per buffer: q, do, then fp32 [3][RT] maximum, log2 of the sum, delta
+  T* const kl = buf0 + NBUF * BUF;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
   const Block blk = block_of(p, (p.Lk + XA_KEYS - 1) / XA_KEYS);
   const int b = blk.b, hk = blk.hk;
@@ -290,58 +306,87 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xa_dkv_kernel(XaParams
   Frag<T, DP> kf, vf;
   kf.load((const T*)p.k + b * p.kb + (long)key * p.kl + hk * p.kh, p.D, h, seen, p.neg);
   vf.load((const T*)p.v + b * p.vb + (long)key * p.vl + hk * p.vh, p.D, h, seen);
+  T* const kl_row = kl + (32 * wid + n) * S + M::E * h;
+  if constexpr (KLDS) {
+#pragma unroll
+    for (int s = 0; s < Frag<T, DP>::S; ++s) *reinterpret_cast<typename M::frag_t*>(kl_row + M::CH * s) = kf.f[s];
+  }
   const float sf = SCALED<T> ? ds_scale(p, b, hk) : 1.f;
   constexpr float P_UP = SCALED<T> ? 15.f : 0.f, P_FACTOR = SCALED<T> ? 32768.f : 1.f;
   const float ds_f = sf / P_FACTOR;
-  const bool any_seen = __any(seen);
+  const bool any_seen = __any(seen), all_seen = __all(seen);
+  const int head_tiles = (p.Lq + RT - 1) / RT;
   // nothing of this workgroup's keys is seen by anyone: its sums are zero
-  const int t0 = blk.z * p.per, t1 = blk.rt * XA_KEYS < len ? min(t0 + p.per, (p.rows + RT - 1) / RT) : t0;
+  const int t0 = blk.z * p.per, t1 = blk.rt * XA_KEYS < len ? min(t0 + p.per, p.G * head_tiles) : t0;
 
   Stage<T, DP, RT> sq, sg;
   float stat = 0.f;   // threads 0 .. 3 RT: one value of the tile's statistics
   const int sw = threadIdx.x / RT, sr = threadIdx.x % RT;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    sq.gather(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
-      const int r = t * RT + row;
-      if (r >= p.rows) return nullptr;
-      const int i = r / p.G, head = hk * p.G + r - i * p.G;
-      return (const T*)p.q + b * p.qb + i * p.ql + head * p.qh;
-    });
-    sg.gather(p.D, [&](int row) __attribute__((always_inline)) -> const T* {
-      const int r = t * RT + row;
-      if (r >= p.rows) return nullptr;
-      const int i = r / p.G, head = hk * p.G + r - i * p.G;
-      return (const T*)p.dout + (((long)b * p.Lq + i) * p.H + head) * p.D;
-    });
-    if (sw < 3) {
-      const int r = t * RT + sr;
-      stat = sw == 1 ? INFINITY : 0.f;   // a row behind the last: P = 0
-      if (r < p.rows) {
-        const int i = r / p.G, head = hk * p.G + r - i * p.G;
-        const long at = ((long)b * p.H + head) * p.Lq + i;
-        stat = sw == 0 ? p.st_m[at] : sw == 1 ? p.st_l[at] : p.delta[at];
-      }
+    const int g = t / head_tiles, i0 = (t - g * head_tiles) * RT, head = hk * p.G + g, left = p.Lq - i0;
+    const T* qp = (const T*)p.q + b * p.qb + i0 * p.ql + head * p.qh;
+    const T* gp = (const T*)p.dout + (((long)b * p.Lq + i0) * p.H + head) * p.D;
+    if (left >= RT) {
+      sq.load(qp, p.ql, p.D);
+      sg.load(gp, (long)p.H * p.D, p.D);
+    } else {
+      auto there = [&](int row) __attribute__((always_inline)) { return row < left; };
+      sq.load_some(qp, p.ql, p.D, there);
+      sg.load_some(gp, (long)p.H * p.D, p.D, there);
     }
+    if (sw < 3) {
+      stat = sw == 1 ? INFINITY : 0.f;   // a row behind the last: P = 0
+      if (sr < left) stat = (sw == 0 ? p.st_m : sw == 1 ? p.st_l : p.delta)[((long)b * p.H + head) * p.Lq + i0 + sr];
+    }
+  };
+  auto store_tile = [&](int t) __attribute__((always_inline)) {
+    T* const to = buf0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    sq.store(to, S);
+    sg.store(to + RT * S, S);
+    if (sw < 3) reinterpret_cast<float*>(to + 2 * RT * S)[sw * RT + sr] = stat;
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;
-  f32x16 dk[DT], dv[DT];
+  f32x16 dk[1][DT], dv[1][DT];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
+  for (int dt = 0; dt < DT; ++dt) dk[0][dt] = zero16(), dv[0][dt] = zero16();
 
-  if (t0 < t1) load_tile(t0);
+  if (t0 < t1) {
+    load_tile(t0);
+    store_tile(t0);
+  }
+  __syncthreads();
   for (int t = t0; t < t1; ++t) {
-    sq.store(qs, S);
-    sg.store(gs, S);
-    if (sw < 3) st[sw * RT + sr] = stat;
-    __syncthreads();
+    const T* const qs = buf0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    const T* const gs = qs + RT * S;
+    const float* const st = reinterpret_cast<const float*>(gs + RT * S);
     if (t + 1 < t1) load_tile(t + 1);
     if (any_seen) {
 #pragma unroll
       for (int u = 0; u < RT / 32; ++u) {
         const int at = (32 * u + n) * S + M::E * h;
-        const f32x16 s = inner<T, DP>(qs + at, kf, zero16());
-        f32x16 pr, dp;
+        float bs[16];
+        if constexpr (BIAS) {
+          const int g = t / head_tiles, i0 = (t - g * head_tiles) * RT + 32 * u, head = hk * p.G + g;
+          const long ba = b * p.bb + head * p.bh + (i0 + 4 * h) * p.bq + key * p.bk;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            bs[k] = 0.f;
+            if (i0 + acc_row(k, h) < p.Lq && seen) {
+              const long e = ba + acc_row(k, 0) * p.bq;
+              bs[k] = p.bias_f32 ? ((const float*)p.bias)[e] : (float)((const T*)p.bias)[e];
+            }
+          }
+        }
+        f32x16 pr = zero16(), dp;
+        if constexpr (KLDS) {
+#pragma unroll
+          for (int s = 0; s < Frag<T, DP>::S; ++s)
+            pr = M::mma(*reinterpret_cast<const typename M::frag_t*>(qs + at + M::CH * s),
+                        *reinterpret_cast<const typename M::frag_t*>(kl_row + M::CH * s), pr);
+        } else {
+          pr = inner<T, DP>(qs + at, kf, pr);
+        }
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
           const f32x4 dl = *reinterpret_cast<const f32x4*>(st + 2 * RT + 32 * u + 8 * run + 4 * h);
@@ -356,25 +401,23 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xa_dkv_kernel(XaParams
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = 4 * run + e;
-            float bs = 0.f;
-            if constexpr (BIAS) {
-              const int r = t * RT + 32 * u + acc_row(k, h);
-              if (r < p.rows && seen) {
-                const int i = r / p.G, head = hk * p.G + r - i * p.G;
-                const long ba = b * p.bb + head * p.bh + i * p.bq + key * p.bk;
-                bs = p.bias_f32 ? ((const float*)p.bias)[ba] : (float)((const T*)p.bias)[ba];
-              }
-            }
-            const float y = exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs) - m[e], LOG2E, P_UP - ll[e])
-                                           : exponent<T>(s[k], c, m[e]) + (P_UP - ll[e]));
-            pr[k] = seen ? y : 0.f;
-            dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
+            pr[k] = exp2_fast(BIAS ? fmaf(fmaf(pr[k], c, bs[k]) - m[e], LOG2E, P_UP - ll[e])
+                                   : exponent<T>(pr[k], c, m[e]) + (P_UP - ll[e]));
           }
         }
-        M::template outer<DT>(gs + 32 * u * S, S, lane, M::pack(pr), dv);
-        M::template outer<DT>(qs + 32 * u * S, S, lane, M::pack(dp), dk);
+        if (!all_seen) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) pr[k] = seen ? pr[k] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
+        const typename M::Packed pv[1] = {M::pack(pr)}, pd[1] = {M::pack(dp)};
+        M::template outer<DT, 1>(gs + 32 * u * S, S, lane, pv, dv);
+        M::template outer<DT, 1>(qs + 32 * u * S, S, lane, pd, dk);
       }
     }
+    if constexpr (NBUF == 1) __syncthreads();
+    if (t + 1 < t1) store_tile(t + 1);
     __syncthreads();
   }
 
@@ -390,8 +433,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xa_dkv_kernel(XaParams
       float x[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = seen ? dk[dt][4 * run + e] * k_scale : 0.f;
-        y[e] = seen ? dv[dt][4 * run + e] * v_scale : 0.f;
+        x[e] = seen ? dk[0][dt][4 * run + e] * k_scale : 0.f;
+        y[e] = seen ? dv[0][dt][4 * run + e] * v_scale : 0.f;
       }
       if (p.splits > 1) {
         store4<float>(p.part + (2l * blk.z * all + at) * p.D + d, x);
@@ -475,8 +518,9 @@ int dq_type(const XaParams& p, hipStream_t st) {
 
 template <typename T, int DP, bool BIAS>
 int dkv_launch(const XaParams& p, hipStream_t st) {
-  constexpr int RT = xa_rt(DP, __is_same(T, float));
-  const size_t lds = (size_t)2 * RT * Mma<T>::row_stride(DP) * sizeof(T) + 3 * RT * 4;
+  constexpr int RT = xa_rt(DP, __is_same(T, float)), S = Mma<T>::row_stride(DP);
+  const size_t lds = buffers<T, false>() * ((size_t)2 * RT * S * sizeof(T) + 3 * RT * 4) +
+                     (keys_in_lds<T, DP>() ? (size_t)XA_KEYS * S * sizeof(T) : 0);
   if (int rc = pf_reserve_lds((const void*)xa_dkv_kernel<T, DP, BIAS>, lds, "xa_dkv_kernel")) return rc;
   const int tiles = (p.Lk + XA_KEYS - 1) / XA_KEYS;
   xa_dkv_kernel<T, DP, BIAS><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);

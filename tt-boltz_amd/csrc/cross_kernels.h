@@ -43,7 +43,7 @@ struct Mma {
   static constexpr int CH = 16, E = 8;
   static constexpr int row_stride(int dp) { return dp + 8; }   // rows land on distinct banks (16 lanes x 16 bytes)
   // only read in transposed 4 x 16 blocks: four rows x 32 channels on distinct banks
-  static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp + 32; }
+  static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp == 64 ? 80 : dp + 32; }
   static PF_DEV f32x16 mma(const frag_t& a, const frag_t& b, const f32x16& c) {
     if constexpr (__is_same(T, half_t)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -72,10 +72,10 @@ struct Mma {
       }
     return c;
   }
-  // acc[dt] += X^T P over 32 rows of the LDS tile X (row stride `st`), taken in P's order.  A transposing
+  // acc[r][dt] += X^T P[r] over 32 rows of the LDS tile X (row stride `st`), taken in P's order.  A transposing
   // read hands lane i of 16 the column i of a 4 x 16 block whose 8-byte pieces the lanes point at.
-  template <int DT>
-  static PF_DEV void outer(const T* x, int st, int lane, const Packed& p, f32x16 (&acc)[DT]) {
+  template <int DT, int R>
+  static PF_DEV void outer(const T* x, int st, int lane, const Packed (&p)[R], f32x16 (&acc)[R][DT]) {
     const int h = lane >> 5, i = lane & 15, c16 = (lane >> 4) & 1;
     const T* at = x + (4 * h + (i >> 2)) * st + 16 * c16 + 4 * (i & 3);
 #pragma unroll
@@ -84,7 +84,8 @@ struct Mma {
       for (int dt = 0; dt < DT; ++dt) {
         const quad_t lo = tr_read(at + (16 * s) * st + 32 * dt), hi = tr_read(at + (16 * s + 8) * st + 32 * dt);
         const frag_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[dt] = mma(a, p.f[s], acc[dt]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][dt] = mma(a, p[r].f[s], acc[r][dt]);
       }
   }
   static PF_DEV quad_t tr_read(const T* p) {
@@ -112,14 +113,17 @@ struct Mma<float> {
     for (int t = 0; t < 16; ++t) c += b[t];
     return c;
   }
-  template <int DT>
-  static PF_DEV void outer(const float* x, int st, int lane, const f32x16& p, f32x16 (&acc)[DT]) {
+  template <int DT, int R>
+  static PF_DEV void outer(const float* x, int st, int lane, const f32x16 (&p)[R], f32x16 (&acc)[R][DT]) {
     const int h = lane >> 5, n = lane & 31;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int k = 0; k < 16; ++k)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[acc_row(r, h) * st + 32 * dt + n], p[r], acc[dt], 0, 0, 0);
+      for (int dt = 0; dt < DT; ++dt) {
+        const float a = x[acc_row(k, h) * st + 32 * dt + n];
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r][k], acc[r][dt], 0, 0, 0);
+      }
   }
 };
 
@@ -146,6 +150,19 @@ PF_DEV f32x16 inner(const T* a, const Frag<T, DP>& b, f32x16 c) {
   for (int s = 0; s < Frag<T, DP>::S; ++s)
     c = Mma<T>::mma(*reinterpret_cast<const typename Mma<T>::frag_t*>(a + Mma<T>::CH * s), b.f[s], c);
   return c;
+}
+
+// c[r] = A B[r]^T over channels: A the LDS tile's 32 rows at `a` (this lane's row, channel E h)
+template <typename T, int DP, int R>
+PF_DEV void inner_rows(const T* a, const Frag<T, DP> (&b)[R], f32x16 (&c)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) c[r] = zero16();
+#pragma unroll
+  for (int s = 0; s < Frag<T, DP>::S; ++s) {
+    const auto f = *reinterpret_cast<const typename Mma<T>::frag_t*>(a + Mma<T>::CH * s);
+#pragma unroll
+    for (int r = 0; r < R; ++r) c[r] = Mma<T>::mma(f, b[r].f[s], c[r]);
+  }
 }
 
 // A tile of ROWS rows x DP channels on its way from global memory to LDS: 16-byte pieces in registers,
@@ -279,20 +296,24 @@ PF_DEV void store4(T* p, const float (&x)[4]) {
 }
 
 // ------------------------------------------------------------------------------ forward
-// FEW = false: 4 waves x 32 rows, every wave over the tile's 64 keys.  FEW = true (at most 32 rows, and
-// few enough tiles): the waves share a 32-row tile and take 32 of the tile's 128 keys each; their
-// results are joined through LDS.
+// FEW = false: every wave over the tile's 64 keys with R tiles of 32 rows.  FEW = true (at most 32 rows): the waves share one
+// 32-row tile and take 32 of the tile's 128 keys each; their results are joined through LDS.
+//
 // LDS buffers of a tile: two, so that a tile needs one barrier, or one where the tiles are large and more
 // workgroups per CU are worth more (single rows stream keys at memory's rate).
 template <typename T, bool FEW>
 constexpr int buffers() { return FEW || __is_same(T, float) ? 1 : 2; }
 
-// Waves per SIMD that a kernel's registers are kept to: two, where 256 registers hold it.
-template <typename T, int DP, bool FEW>
-constexpr int waves() { return DP == 128 && (FEW || __is_same(T, float)) ? 1 : 2; }
+// Waves per SIMD that the forward kernel's registers are kept to.
+template <typename T, int DP, bool BIAS, bool FEW, int R>
+constexpr int fwd_waves() {
+  if (DP == 128) return FEW || __is_same(T, float) ? 1 : 2;
+  if (R == 2) return 2;
+  return __is_same(T, float) ? 2 : DP == 64 ? (BIAS || FEW ? 3 : 4) : 4;
+}
 
-template <typename T, int DP, bool BIAS, bool FEW>
-__global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaParams p) {
+template <typename T, int DP, bool BIAS, bool FEW, int R>
+__global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fwd_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP), VS = M::col_stride(DP);
@@ -300,17 +321,23 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
   constexpr int BUF = KT * (KS + VS), NBUF = buffers<T, FEW>();
   T* const ks0 = reinterpret_cast<T*>(smem);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
-  constexpr int ROWS = FEW ? 32 : 128;
+  constexpr int ROWS = FEW ? 32 : 128 * R;
   const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
   const int b = blk.b, hk = blk.hk;
-  const int r = blk.rt * ROWS + (FEW ? 0 : 32 * wid) + n;
-  const bool row_ok = r < p.rows;
-  const int i = row_ok ? r / p.G : 0, head = hk * p.G + (row_ok ? r - i * p.G : 0);
   const int sub0 = FEW ? 32 * wid : 0;
-  Frag<T, DP> q;
-  q.load((const T*)p.q + b * p.qb + i * p.ql + head * p.qh, p.D, h, row_ok, p.neg);
-  const char* bias = nullptr;
-  if constexpr (BIAS) bias = bias_row<T>(p, b, head, i);
+  int row[R], i[R], head[R];   // a lane's rows
+  bool row_ok[R];
+  Frag<T, DP> q[R];
+  const char* bias[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    row[r] = blk.rt * ROWS + (FEW ? 0 : 32 * (R * wid + r)) + n;
+    row_ok[r] = row[r] < p.rows;
+    i[r] = row_ok[r] ? row[r] / p.G : 0;
+    head[r] = hk * p.G + (row_ok[r] ? row[r] - i[r] * p.G : 0);
+    q[r].load((const T*)p.q + b * p.qb + i[r] * p.ql + head[r] * p.qh, p.D, h, row_ok[r], p.neg);
+    if constexpr (BIAS) bias[r] = bias_row<T>(p, b, head[r], i[r]);
+  }
   const int len = length_of(p, b);
   const int t0 = blk.z * p.per, t1 = min(t0 + p.per, (len + KT - 1) / KT);
   const uint8_t* mask = p.mask ? p.mask + b * p.mb : nullptr;
@@ -319,17 +346,21 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
 
   Stage<T, DP, KT> sk, sv;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    load_keys<T, DP, KT>(sk, kb, p.kl, p.D, t, len, mask);
-    load_keys<T, DP, KT>(sv, vb, p.vl, p.D, t, len, mask);
+    load_keys(sk, kb, p.kl, p.D, t, len, mask);
+    load_keys(sv, vb, p.vl, p.D, t, len, mask);
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;   // x in units of 1 (bias) or log2
   // the reference of the exponentials follows the maximum when that has grown by SLACK: p <= 2^8
   constexpr float SLACK = BIAS ? 5.f : 8.f;
-  float m = -INFINITY, l = 0.f;                       // l: this lane's half of the keys
-  f32x16 o[DT];
+  float m[R], l[R];                                   // l: this lane's half of the keys
+  f32x16 o[R][DT];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[r][dt] = zero16();
+  }
 
   if (t0 < t1) {
     load_tile(t0);
@@ -348,54 +379,69 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
       word = __ballot(key_l < len && (!mask || mask[key_l]));
     }
     if (word) {
-      float x[NSUB][16];
-      float mx = -INFINITY;
+      f32x16 x[NSUB][R];
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
-        float bs[4][4];
+        float bs[R][4][4];
         if constexpr (BIAS) {
 #pragma unroll
-          for (int run = 0; run < 4; ++run)
-            load_bias<T>(p, bias, t * KT + sub0 + 32 * u + 8 * run + 4 * h, row_ok, bs[run]);
-        }
-        const f32x16 s = inner<T, DP>(ks + (sub0 + 32 * u + n) * KS + M::E * h, q, zero16());
+          for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) x[u][k] = BIAS ? fmaf(s[k], c, bs[k >> 2][k & 3]) : s[k];
+            for (int run = 0; run < 4; ++run)
+              load_bias<T>(p, bias[r], t * KT + sub0 + 32 * u + 8 * run + 4 * h, row_ok[r], bs[r][run]);
+        }
+        inner_rows<T, DP, R>(ks + (sub0 + 32 * u + n) * KS + M::E * h, q, x[u]);
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[u][r][k] = fmaf(x[u][r][k], c, bs[r][k >> 2][k & 3]);
+        }
         const uint32_t w = (uint32_t)(word >> (FEW ? 0 : 32 * u));
         if (w != 0xffffffffu) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[u][k] = (w >> (4 * h) >> acc_row(k, 0)) & 1 ? x[u][k] : -INFINITY;
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[u][r][k] = (w >> (4 * h) >> acc_row(k, 0)) & 1 ? x[u][r][k] : -INFINITY;
         }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, x[u][k]);
       }
-      mx = xor32_max(mx);
-      if (!BIAS) mx *= c;
-      if (__any(mx > m + SLACK)) {
-        const float m_new = fmaxf(m, mx);
-        const float a = m_new > m ? exp2_fast(BIAS ? (m - m_new) * LOG2E : m - m_new) : 1.f;
-        l *= a;
+      typename M::Packed pk[NSUB][R];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+      for (int r = 0; r < R; ++r) {
+        float mx = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[dt][k] *= a;
-        m = m_new;
-      }
-      const float mu = m == -INFINITY ? 0.f : m;   // nothing seen so far: every p is 0
+        for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u) {
-        f32x16 pr;
+          for (int k = 0; k < 16; ++k) mx = fmaxf(mx, x[u][r][k]);
+        mx = xor32_max(mx);
+        if (!BIAS) mx *= c;
+        if (__any(mx > m[r] + SLACK)) {
+          const float m_new = fmaxf(m[r], mx);
+          const float a = m_new > m[r] ? exp2_fast(BIAS ? (m[r] - m_new) * LOG2E : m[r] - m_new) : 1.f;
+          l[r] *= a;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) pr[k] = exp2_fast(BIAS ? (x[u][k] - mu) * LOG2E : exponent<T>(x[u][k], c, mu));
-        const typename M::Packed pk = M::pack(pr);
-        if constexpr (BIAS) {   // the bias's gradient wants P, and so the sum, to fp32
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int k = 0; k < 16; ++k) l += pr[k];
-        } else {
-          l = M::sum(pk, l);
+            for (int k = 0; k < 16; ++k) o[r][dt][k] *= a;
+          m[r] = m_new;
         }
-        M::template outer<DT>(vs + (sub0 + 32 * u) * VS, VS, lane, pk, o);
+        const float mu = m[r] == -INFINITY ? 0.f : m[r];   // nothing seen so far: every p is 0
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
+          f32x16 pr;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) pr[k] = exp2_fast(BIAS ? (x[u][r][k] - mu) * LOG2E : exponent<T>(x[u][r][k], c, mu));
+          pk[u][r] = M::pack(pr);
+          if constexpr (BIAS) {   // the bias's gradient wants P, and so the sum, to fp32
+#pragma unroll
+            for (int k = 0; k < 16; ++k) l[r] += pr[k];
+          } else {
+            l[r] = M::sum(pk[u][r], l[r]);
+          }
+        }
       }
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u) M::template outer<DT, R>(vs + (sub0 + 32 * u) * VS, VS, lane, pk[u], o);
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) {
@@ -405,7 +451,10 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
     }
     __syncthreads();
   }
-  l = xor32_sum(l);
+#pragma unroll
+  for (int r = 0; r < R; ++r) l[r] = xor32_sum(l[r]);
+  const long part_rows = (long)p.splits * p.B * p.Hk * p.rows;
+  const long part_row0 = ((long)blk.z * p.B * p.Hk + (long)b * p.Hk + hk) * p.rows;
 
   if constexpr (FEW) {
     // join the four waves: their maxima and sums, then thread (row, 4 channels) adds the four parts
@@ -416,40 +465,38 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int run = 0; run < 4; ++run) {
-        const f32x4 v = {o[dt][4 * run], o[dt][4 * run + 1], o[dt][4 * run + 2], o[dt][4 * run + 3]};
+        const f32x4 v = {o[0][dt][4 * run], o[0][dt][4 * run + 1], o[0][dt][4 * run + 2], o[0][dt][4 * run + 3]};
         *reinterpret_cast<f32x4*>(os + (32 * wid + n) * OS + 32 * dt + 8 * run + 4 * h) = v;
       }
     if (h == 0) {
-      ms[(32 * wid + n) * 2] = m;
-      ms[(32 * wid + n) * 2 + 1] = l;
+      ms[(32 * wid + n) * 2] = m[0];
+      ms[(32 * wid + n) * 2 + 1] = l[0];
     }
     __syncthreads();
-    const int row = threadIdx.x >> 3, sub = threadIdx.x & 7, rr = blk.rt * ROWS + row;
+    const int tr = threadIdx.x >> 3, sub = threadIdx.x & 7, rr = blk.rt * ROWS + tr;
     if (rr >= p.rows) return;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ms[(32 * w + row) * 2]);
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ms[(32 * w + tr) * 2]);
     float f[4], ll = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = ms[(32 * w + row) * 2];
+      // (a wave that saw nothing has sums of 0, or NaN where its scores were: that has to spread)
+      const float mw = ms[(32 * w + tr) * 2];
       f[w] = mw == -INFINITY ? 0.f : exp2_fast(BIAS ? (mw - mm) * LOG2E : mw - mm);
-      ll += f[w] * ms[(32 * w + row) * 2 + 1];
+      ll += f[w] * ms[(32 * w + tr) * 2 + 1];
     }
-    // (a wave that saw nothing has sums of 0, or NaN where its scores were: they must spread)
     const int ri = rr / p.G, rh = hk * p.G + rr - ri * p.G;
     const long row_at = ((long)b * p.Lq + ri) * p.H + rh;
     const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-    const long part_row = ((long)blk.z * p.B * p.Hk + (long)b * p.Hk + hk) * p.rows + rr;
-    const long part_rows = (long)p.splits * p.B * p.Hk * p.rows;
     for (int d = 4 * sub; d < p.D; d += 32) {
       float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] += f[w] * os[(32 * w + row) * OS + d + e];
+        for (int e = 0; e < 4; ++e) a[e] += f[w] * os[(32 * w + tr) * OS + d + e];
       if (p.splits > 1) {
-        store4<float>(p.part + part_row * p.D + d, a);
+        store4<float>(p.part + (part_row0 + rr) * p.D + d, a);
         continue;
       }
 #pragma unroll
@@ -459,8 +506,8 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
     }
     if (sub == 0) {
       if (p.splits > 1) {
-        p.part[part_rows * p.D + 2 * part_row] = mm;
-        p.part[part_rows * p.D + 2 * part_row + 1] = ll;
+        p.part[part_rows * p.D + 2 * (part_row0 + rr)] = mm;
+        p.part[part_rows * p.D + 2 * (part_row0 + rr) + 1] = ll;
       } else if (p.st_m) {
         const long at = ((long)b * p.H + rh) * p.Lq + ri;
         p.st_m[at] = mm == -INFINITY ? 0.f : mm;
@@ -468,35 +515,36 @@ __global__ __launch_bounds__(256, (waves<T, DP, FEW>())) void xa_fwd_kernel(XaPa
       }
     }
   } else {
-    if (!row_ok) return;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const long row_at = ((long)b * p.Lq + i) * p.H + head;
-    const long part_row = ((long)blk.z * p.B * p.Hk + (long)b * p.Hk + hk) * p.rows + r;
-    const long part_rows = (long)p.splits * p.B * p.Hk * p.rows;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int r = 0; r < R; ++r) {
+      if (!row_ok[r]) continue;
+      const float inv = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
+      const long row_at = ((long)b * p.Lq + i[r]) * p.H + head[r];
 #pragma unroll
-      for (int run = 0; run < 4; ++run) {
-        const int d = 32 * dt + 8 * run + 4 * h;
-        if (d >= p.D) continue;
-        float a[4];
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = o[dt][4 * run + e] * (p.splits > 1 ? 1.f : inv);
-        if (p.splits > 1) {
-          store4<float>(p.part + part_row * p.D + d, a);
-        } else {
-          store4<T>((T*)p.o + row_at * p.D + d, a);
-          if (p.o32) store4<float>(p.o32 + row_at * p.D + d, a);
+        for (int run = 0; run < 4; ++run) {
+          const int d = 32 * dt + 8 * run + 4 * h;
+          if (d >= p.D) continue;
+          float a[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = o[r][dt][4 * run + e] * (p.splits > 1 ? 1.f : inv);
+          if (p.splits > 1) {
+            store4<float>(p.part + (part_row0 + row[r]) * p.D + d, a);
+          } else {
+            store4<T>((T*)p.o + row_at * p.D + d, a);
+            if (p.o32) store4<float>(p.o32 + row_at * p.D + d, a);
+          }
         }
-      }
-    if (h == 0) {
-      if (p.splits > 1) {
-        p.part[part_rows * p.D + 2 * part_row] = m;
-        p.part[part_rows * p.D + 2 * part_row + 1] = l;
-      } else if (p.st_m) {
-        const long at = ((long)b * p.H + head) * p.Lq + i;
-        p.st_m[at] = m == -INFINITY ? 0.f : m;
-        p.st_l[at] = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+      if (h == 0) {
+        if (p.splits > 1) {
+          p.part[part_rows * p.D + 2 * (part_row0 + row[r])] = m[r];
+          p.part[part_rows * p.D + 2 * (part_row0 + row[r]) + 1] = l[r];
+        } else if (p.st_m) {
+          const long at = ((long)b * p.H + head[r]) * p.Lq + i[r];
+          p.st_m[at] = m[r] == -INFINITY ? 0.f : m[r];
+          p.st_l[at] = l[r] == 0.f ? INFINITY : __builtin_amdgcn_logf(l[r]);
+        }
       }
     }
   }
@@ -547,12 +595,13 @@ size_t fwd_lds() {
   return tiles > join ? tiles : join;
 }
 
-template <typename T, int DP, bool BIAS, bool FEW>
+template <typename T, int DP, bool BIAS, bool FEW, int R>
 int fwd_launch(const XaParams& p, hipStream_t st) {
   const size_t lds = fwd_lds<T, DP, FEW>();
-  if (int rc = pf_reserve_lds((const void*)xa_fwd_kernel<T, DP, BIAS, FEW>, lds, "xa_fwd_kernel")) return rc;
-  const int tiles = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
-  xa_fwd_kernel<T, DP, BIAS, FEW><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
+  if (int rc = pf_reserve_lds((const void*)xa_fwd_kernel<T, DP, BIAS, FEW, R>, lds, "xa_fwd_kernel")) return rc;
+  constexpr int ROWS = FEW ? 32 : 128 * R;
+  const int tiles = (p.rows + ROWS - 1) / ROWS;
+  xa_fwd_kernel<T, DP, BIAS, FEW, R><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
   PF_CHECK_LAUNCH("xa_fwd_kernel");
   if (p.splits > 1) {
     const long threads = (long)p.B * p.Hk * p.rows * (p.D / 4);
@@ -564,8 +613,12 @@ int fwd_launch(const XaParams& p, hipStream_t st) {
 
 template <typename T, int DP>
 int fwd_dp(const XaParams& p, hipStream_t st) {
-  if (p.bias) return p.few ? fwd_launch<T, DP, true, true>(p, st) : fwd_launch<T, DP, true, false>(p, st);
-  return p.few ? fwd_launch<T, DP, false, true>(p, st) : fwd_launch<T, DP, false, false>(p, st);
+  if (p.bias) return p.few ? fwd_launch<T, DP, true, true, 1>(p, st) : fwd_launch<T, DP, true, false, 1>(p, st);
+  if (p.few) return fwd_launch<T, DP, false, true, 1>(p, st);
+  if constexpr (DP == 64 && sizeof(T) == 2) {
+    if (p.wide) return fwd_launch<T, DP, false, false, 2>(p, st);
+  }
+  return fwd_launch<T, DP, false, false, 1>(p, st);
 }
 
 template <typename T>
