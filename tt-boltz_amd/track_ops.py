@@ -1,10 +1,11 @@
 """Operators between tracks in the caller's own element type, with their gradients.
 
-``cross_attention`` (queries of one track over another track's keys and values), ``embedding`` (token -> atom broadcasts, residue types, vocabularies) with ``embedding_grad`` (its
-transpose: sums by token) and ``dropout_add`` (the pair updates' residual dropout) take fp32, fp16 or
-bf16 device tensors and return the same type; sums and statistics are fp32.  They differentiate like
-torch's own operators (``cross_attention`` once).  The ``launch_*`` functions enqueue the kernels on the
-current stream, for programs that write their own backward pass or capture one: they take contiguous
+``cross_attention`` (queries of one track over another track's keys and values), ``embedding`` (token ->
+atom broadcasts, residue types, vocabularies) with ``embedding_grad`` (its transpose: sums by token) and
+``dropout_add`` (the pair updates' residual dropout) take fp32, fp16 or bf16 device tensors and return the
+same type; sums and statistics are fp32.  They differentiate like torch's own operators
+(``cross_attention`` once).  The ``launch_*`` functions enqueue the kernels on the current stream of the
+current device, for programs that write their own backward pass or capture one: they take contiguous
 device tensors and allocate nothing.
 
 Under ``torch.cuda.graph`` the same care is due as with torch's operators: ``backward()`` captured
@@ -14,11 +15,9 @@ first, use ``torch.autograd.grad``, or call the ``launch_*`` functions.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-import math
 import operator
-from typing import Optional, Tuple, Union
+from typing import Optional, Union
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -34,17 +33,22 @@ SHARED_CODE = {None: 0, "row": 1, "column": 2}                         # PF_DROP
 # --------------------------------------------------------------------------------------
 def _device(what: str, *ts: Optional[torch.Tensor]) -> torch.device:
     """The one device of the given tensors, RuntimeError where they are on several or not on a GPU."""
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f"{what}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
-    return ops._require_gpu(*ts)
+    dev = None
+    for t in ts:
+        if t is not None:
+            d = t.device
+            if dev is None:
+                dev = d
+                if d.type != "cuda":
+                    ops._require_gpu(t)
+            elif d != dev:
+                raise RuntimeError(f"{what}: tensors on different devices ({dev}, {d})")
+    return dev
 
 
-def _on(device: torch.device):
-    """The device made current for a launch (its current stream is the one used), where it is not."""
-    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _elsewhere(device: torch.device) -> bool:
+    """Whether ``device`` is not the current one: its own current stream is the one to launch on."""
+    return device.type == "cuda" and device.index != torch._C._cuda_getDevice()
 
 
 def _code(what: str, t: torch.Tensor) -> int:
@@ -54,52 +58,70 @@ def _code(what: str, t: torch.Tensor) -> int:
     return code
 
 
+# (the functions below run under autograd.Function or where nothing wants a gradient: no detach)
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous values of ``t``, without its graph."""
-    t = t.detach()
+    """Contiguous values of ``t``."""
     return (t.resolve_neg() if t.is_neg() else t).contiguous()
 
 
 def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # --------------------------------------------------------------------------------------
 # cross attention
 # --------------------------------------------------------------------------------------
 def _strided(t: torch.Tensor) -> torch.Tensor:
-    """``t`` where the kernels can read it in 16-byte pieces of its last dimension, else a copy."""
-    t = t.detach()
-    unit = 16 // t.element_size()
-    if (t.is_neg() or t.data_ptr() % 16 or (t.shape[-1] > 1 and t.stride(-1) != 1)
-            or any(s % unit for n, s in zip(t.shape[:-1], t.stride()) if n > 1)):
-        t = t.resolve_neg().clone(memory_format=torch.contiguous_format)
+    """``t`` [., ., ., D] where the kernels can read it in 16-byte pieces of its last dimension, else a copy."""
+    s0, s1, s2, s3 = t.stride()
+    unit = 3 if t.dtype == torch.float32 else 7
+    if s3 == 1 and not (s0 | s1 | s2) & unit and not t.data_ptr() & 15 and not t.is_neg():
+        return t
+    if (t.is_neg() or t.data_ptr() & 15 or s3 != 1
+            or any(s & unit for n, s in zip(t.shape, (s0, s1, s2)) if n > 1)):
+        return t.resolve_neg().clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     t = _dense(t)
-    return t.clone() if t.data_ptr() % 16 else t
+    return t.clone() if t.data_ptr() & 15 else t
 
 
-def _strides(t: torch.Tensor, dims) -> list:
-    return [t.stride(d) if t.shape[d] > 1 else 0 for d in dims]
+def _strides(t: torch.Tensor) -> tuple:
+    """Strides of the leading three dimensions; those of size 1 (any number stands there) as 0."""
+    s = t.stride()
+    if 1 in t.shape:
+        return tuple(0 if n == 1 else x for n, x in zip(t.shape[:3], s))
+    return s[:3]
 
 
 def _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats) -> "_lib.CrossAttnArgs":
     (B, Lq, H, D), (_, Lk, Hk, _) = q.shape, k.shape
-    a = _lib.CrossAttnArgs(B, Lq, Lk, H, Hk, D, DTYPE_CODE[q.dtype], 0 if bias is None else DTYPE_CODE[bias.dtype], scale,
-                           q.data_ptr(), *_strides(q, (0, 1, 2)), k.data_ptr(), *_strides(k, (0, 1, 2)),
-                           v.data_ptr(), *_strides(v, (0, 1, 2)))
-    if bias is not None:
-        a.bias = bias.data_ptr()
-        a.bias_b, a.bias_h, a.bias_q, a.bias_k = _strides(bias, (0, 1, 2, 3))
-        if Lk == 1:
-            a.bias_k = 1
-    if mask is not None:
-        a.mask, a.mask_b = mask.data_ptr(), mask.stride(0) if B > 1 else 0
-    a.k_lens, a.o, a.o32, a.stats = ops._ptr(k_lens), ops._ptr(o), ops._ptr(o32), ops._ptr(stats)
-    return a
+    if bias is None:
+        bias_code, bias_at, bias_strides = 0, None, (0, 0, 0, 0)
+    else:
+        bias_code, bias_at = DTYPE_CODE[bias.dtype], bias.data_ptr()
+        bias_strides = (*_strides(bias), bias.stride(3) if Lk > 1 else 1)
+    return _lib.CrossAttnArgs(
+        B, Lq, Lk, H, Hk, D, DTYPE_CODE[q.dtype], bias_code, scale, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k),
+        v.data_ptr(), *_strides(v), bias_at, *bias_strides, None if mask is None else mask.data_ptr(),
+        0 if mask is None or B == 1 else mask.stride(0), ops._ptr(k_lens), ops._ptr(o), ops._ptr(o32), ops._ptr(stats),
+        None, 0, ops._stream())
+
+
+def _with_workspace(a, size: str, device: torch.device):
+    """The call's scratch memory (kept by the caller until the call is enqueued)."""
+    nb = getattr(_lib.load(), size)(ctypes.byref(a))
+    if nb:
+        ws = ops.workspace(nb, device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nb
+        return ws
+    return None
 
 
 def launch_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
@@ -112,7 +134,8 @@ def launch_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o:
     types) and ``stats`` fp32 [2, B, H, Lq] keep what the backward pass needs; ``ws`` of
     ``cross_attention_workspace_bytes``.  (With a bias gradient, 16-bit types need no ``o32``.)"""
     a = _cross_args(q, k, v, bias, mask, k_lens, q.shape[-1] ** -0.5 if scale is None else scale, o, o32, stats)
-    a.workspace, a.workspace_bytes, a.stream = ops._ptr(ws), 0 if ws is None else ws.numel(), ops._stream()
+    if ws is not None:
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _lib.check(_lib.load().pf_cross_attn_fwd(ctypes.byref(a)), "pf_cross_attn_fwd")
 
 
@@ -120,17 +143,20 @@ def cross_attention_workspace_bytes(q: torch.Tensor, k: torch.Tensor) -> int:
     return _lib.load().pf_cross_attn_workspace_size(ctypes.byref(_cross_args(q, k, k, None, None, None, 1.0, None, None, None)))
 
 
-def _bwd_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats, dbias_shape):
-    a = _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats)
-    if dbias_shape is not None:
-        a.dbias_B, a.dbias_H = dbias_shape[:2]
-    return a
-
-
 def cross_attention_bwd_workspace_bytes(q: torch.Tensor, k: torch.Tensor, bias: Optional[torch.Tensor] = None) -> int:
     """``bias``: the bias whose gradient is wanted, or None."""
-    a = _bwd_args(q, k, k, bias, None, None, 1.0, None, None, None, None if bias is None else bias.shape)
+    a = _cross_args(q, k, k, bias, None, None, 1.0, None, None, None)
+    if bias is not None:
+        a.dbias_B, a.dbias_H = bias.shape[:2]
     return _lib.load().pf_cross_attn_bwd_workspace_size(ctypes.byref(a))
+
+
+def _bwd_args(do, q, k, v, o, o32, stats, dq, dk, dv, bias, dbias, mask, k_lens, scale):
+    a = _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats)
+    a.dout, a.dq, a.dk, a.dv, a.dbias = ops._ptr(do), ops._ptr(dq), ops._ptr(dk), ops._ptr(dv), ops._ptr(dbias)
+    if dbias is not None:
+        a.dbias_B, a.dbias_H = dbias.shape[:2]
+    return a
 
 
 def launch_cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -141,32 +167,52 @@ def launch_cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tenso
                                k_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> None:
     """The gradients of ``launch_cross_attention`` (pf_cross_attn_bwd) into contiguous dq, dk, dv and
     dbias (of bias's shape and type); dq alone, or dk and dv alone, where the others are None."""
-    a = _bwd_args(q, k, v, bias, mask, k_lens, q.shape[-1] ** -0.5 if scale is None else scale, o, o32, stats,
-                  None if dbias is None else dbias.shape)
-    a.dout, a.dq, a.dk, a.dv, a.dbias = ops._ptr(do), ops._ptr(dq), ops._ptr(dk), ops._ptr(dv), ops._ptr(dbias)
-    a.workspace, a.workspace_bytes, a.stream = ops._ptr(ws), ws.numel(), ops._stream()
+    a = _bwd_args(do, q, k, v, o, o32, stats, dq, dk, dv, bias, dbias, mask, k_lens,
+                  q.shape[-1] ** -0.5 if scale is None else scale)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _lib.check(_lib.load().pf_cross_attn_bwd(ctypes.byref(a)), "pf_cross_attn_bwd")
 
 
-def _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep: bool, keep_o: bool = False):
-    """(o, o32, stats) on prepared tensors; the last two only where a backward pass will read them."""
+def _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep: bool, keep_o: bool):
+    """(o, o32, stats) on strided tensors; the last two only where a backward pass will read them."""
     dev = q.device
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    o32 = torch.empty(q.shape, dtype=torch.float32, device=dev) if keep_o and q.dtype != torch.float32 else None
-    stats = torch.empty((2, q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev) if keep else None
-    with _on(dev):
-        nb = cross_attention_workspace_bytes(q, k)
-        launch_cross_attention(q, k, v, o, bias, mask, k_lens, scale, o32, stats, ops.workspace(nb, dev) if nb else None)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep, keep_o)
+    shape = q.shape
+    o = torch.empty(shape, dtype=q.dtype, device=dev)
+    o32 = torch.empty(shape, dtype=torch.float32, device=dev) if keep_o and q.dtype != torch.float32 else None
+    stats = torch.empty((2, shape[0], shape[2], shape[1]), dtype=torch.float32, device=dev) if keep else None
+    a = _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats)
+    ws = _with_workspace(a, "pf_cross_attn_workspace_size", dev)  # noqa: F841
+    _lib.check(_lib.load().pf_cross_attn_fwd(ctypes.byref(a)), "pf_cross_attn_fwd")
     return o, o32, stats
+
+
+def _cross_bwd(do, q, k, v, bias, mask, k_lens, o32, stats, scale, want_q: bool, want_kv: bool, want_b: bool):
+    dev = q.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _cross_bwd(do, q, k, v, bias, mask, k_lens, o32, stats, scale, want_q, want_kv, want_b)
+    some = q.numel() > 0 and k.numel() > 0   # else nothing is launched, and what has elements is zero
+    make = torch.empty if some else torch.zeros
+    dq = make(q.shape, dtype=q.dtype, device=dev) if want_q or want_b else None
+    dk, dv = (make(k.shape, dtype=q.dtype, device=dev) if want_kv else None for _ in range(2))
+    dbias = make(bias.shape, dtype=bias.dtype, device=dev) if want_b else None
+    if some:
+        do = _aligned(do)   # (held by name until the launch: a pointer keeps nothing alive)
+        a = _bwd_args(do, q, k, v, o32, o32, stats, dq, dk, dv, bias, dbias, mask, k_lens, scale)
+        ws = _with_workspace(a, "pf_cross_attn_bwd_workspace_size", dev)  # noqa: F841
+        _lib.check(_lib.load().pf_cross_attn_bwd(ctypes.byref(a)), "pf_cross_attn_bwd")
+    return dq, dk, dv, dbias
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, mask, k_lens, scale):
-        qs, ks, vs = _strided(q), _strided(k), _strided(v)
-        b = None if bias is None else bias.detach()
+        q, k, v = _strided(q), _strided(k), _strided(v)
         # (a bias gradient of 16-bit types does without the unrounded o)
-        o, o32, stats = _cross_fwd(qs, ks, vs, b, mask, k_lens, scale, True, not ctx.needs_input_grad[3])
+        o, o32, stats = _cross_fwd(q, k, v, bias, mask, k_lens, scale, True, not ctx.needs_input_grad[3])
         ctx.save_for_backward(q, k, v, bias, mask, k_lens, o if q.dtype == torch.float32 else o32, stats)
         ctx.scale = scale
         return o
@@ -176,18 +222,7 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, grad):
         q, k, v, bias, mask, k_lens, o32, stats = ctx.saved_tensors
         want_q, want_k, want_v, want_b = ctx.needs_input_grad[:4]
-        q, k, v, do = _strided(q), _strided(k), _strided(v), _aligned(grad)
-        bias = None if bias is None else bias.detach()
-        dev = q.device
-        some = q.numel() > 0 and k.numel() > 0   # else nothing is launched, and what has elements is zero
-        make = torch.empty if some else torch.zeros
-        dq = make(q.shape, dtype=q.dtype, device=dev) if want_q or want_b else None
-        dk, dv = (make(k.shape, dtype=q.dtype, device=dev) if want_k or want_v else None for _ in range(2))
-        dbias = make(bias.shape, dtype=bias.dtype, device=dev) if want_b else None
-        if some:
-            with _on(dev):
-                ws = ops.workspace(cross_attention_bwd_workspace_bytes(q, k, bias if want_b else None), dev)
-                launch_cross_attention_bwd(do, q, k, v, o32, o32, stats, dq, dk, dv, ws, bias, dbias, mask, k_lens, ctx.scale)
+        dq, dk, dv, dbias = _cross_bwd(grad, q, k, v, bias, mask, k_lens, o32, stats, ctx.scale, want_q, want_k or want_v, want_b)
         return dq if want_q else None, dk if want_k else None, dv if want_v else None, dbias, None, None, None
 
 
@@ -225,7 +260,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Opt
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"cross_attention: D must be a multiple of 8 up to 128, got {D}")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or abs(scale) > 3e38:
+    if not abs(scale) <= 3e38:
         raise ValueError(f"cross_attention: scale must be finite, got {scale}")
     if bias is not None:
         if bias.dim() > 4 or bias.dim() < 2:
@@ -251,8 +286,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Opt
         k_lens = k_lens.contiguous()
     if _wants_grad(q, k, v, bias):
         return _CrossAttention.apply(q, k, v, bias, mask, k_lens, scale)
-    return _cross_fwd(_strided(q), _strided(k), _strided(v), None if bias is None else bias.detach(), mask, k_lens, scale,
-                      False)[0]
+    return _cross_fwd(_strided(q), _strided(k), _strided(v), bias, mask, k_lens, scale, False, False)[0]
 
 
 # --------------------------------------------------------------------------------------
@@ -286,15 +320,17 @@ def _index(what: str, index: torch.Tensor) -> torch.Tensor:
     return index.contiguous()
 
 
-def _embedding(index: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
-    C = weight.shape[1]
-    w = weight.detach()
+def _embedding(index: torch.Tensor, w: torch.Tensor, scale: float) -> torch.Tensor:
+    dev = w.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _embedding(index, w, scale)
+    V, C = w.shape
     # rows are read where they are; other strides through a copy
-    if w.is_neg() or (C > 1 and w.stride(1) != 1) or (w.shape[0] > 1 and w.stride(0) < C):
+    if w.is_neg() or (C > 1 and w.stride(1) != 1) or (V > 1 and w.stride(0) < C):
         w = _dense(w)
-    out = torch.empty((*index.shape, C), dtype=w.dtype, device=w.device)
-    with _on(w.device):
-        launch_embedding(index, w, out, scale)
+    out = torch.empty((*index.shape, C), dtype=w.dtype, device=dev)
+    launch_embedding(index, w, out, scale)
     return out
 
 
@@ -330,12 +366,15 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> 
 
 
 def _embedding_grad(grad: torch.Tensor, index: torch.Tensor, num_rows: int, scale: float) -> torch.Tensor:
+    dev = grad.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _embedding_grad(grad, index, num_rows, scale)
     grad = _dense(grad)
     C = grad.shape[-1]
-    dw = torch.empty((num_rows, C), dtype=grad.dtype, device=grad.device)
-    with _on(grad.device):
-        ws = ops.workspace(embedding_grad_workspace_bytes(index.numel(), num_rows, C), grad.device)
-        launch_embedding_grad(index, grad, dw, ws, scale)
+    dw = torch.empty((num_rows, C), dtype=grad.dtype, device=dev)
+    ws = ops.workspace(embedding_grad_workspace_bytes(index.numel(), num_rows, C), dev)
+    launch_embedding_grad(index, grad, dw, ws, scale)
     return dw
 
 
@@ -384,20 +423,24 @@ def launch_dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], out: t
     else:
         I, J, C = x.shape[-3:]
         B = x.numel() // (I * J * C) if x.numel() else 0
-    on_device = isinstance(seed, torch.Tensor)
-    a = _lib.DropoutArgs(B=B, I=I, J=J, C=C, dtype=DTYPE_CODE[x.dtype], shared=SHARED_CODE[shared], p=p,
-                         seed=0 if on_device else seed & 0xFFFFFFFFFFFFFFFF, offset=offset,
-                         seed_at=ops._ptr(seed) if on_device else None, x=ops._ptr(x), residual=ops._ptr(residual),
-                         out=ops._ptr(out), stream=ops._stream())
+    if isinstance(seed, torch.Tensor):
+        seed, seed_at = 0, seed.data_ptr()
+    else:
+        seed, seed_at = seed & 0xFFFFFFFFFFFFFFFF, None
+    a = _lib.DropoutArgs(B, I, J, C, DTYPE_CODE[x.dtype], SHARED_CODE[shared], p, seed, offset, seed_at, x.data_ptr(),
+                         ops._ptr(residual), out.data_ptr(), ops._stream())
     _lib.check(_lib.load().pf_dropout_add_fwd(ctypes.byref(a)), "pf_dropout_add_fwd")
 
 
 def _dropout_add(x, residual, p, seed, offset, shared):
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _dropout_add(x, residual, p, seed, offset, shared)
     x = _dense(x)
     residual = None if residual is None else _dense(residual)
     out = torch.empty_like(x)
-    with _on(x.device):
-        launch_dropout_add(x, residual, out, p, seed, offset, shared)
+    launch_dropout_add(x, residual, out, p, seed, offset, shared)
     return out
 
 
