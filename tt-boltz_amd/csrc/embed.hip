@@ -7,13 +7,12 @@
 //
 // The gradient reads every row of g once and writes every row of dw once, in fp32 sums whose order
 // depends on the tokens alone (no float atomics: the same call gives the same bits).  Tokens are
-// radix-sorted with their positions (stable, integer ranks), then
-//   * embed_grad_kernel, part 1: a table row that at most CH of the sorted tokens name is summed and
-//     written by one group of lanes (zeros where no token names it);
-//   * part 2: the sorted list is cut into chunks of CH; where a row's run is longer than CH, each
-//     chunk's part of it is summed into a workspace row (a chunk meets at most two such runs: one
-//     that holds its first token and one that holds its last);
-//   * embed_join_kernel adds a long run's parts, in the chunks' order.
+// radix-sorted with their positions (stable, integer ranks) and cut into chunks; then
+//   * embed_grad_kernel, part 1: a group of lanes streams a chunk's rows and writes a table row where the
+//     token changes.  A run of one token that crosses a chunk's border goes to a workspace row instead (at
+//     most two a chunk: the run that came in, the run that goes out);
+//   * part 2: the rows that no token names get their zeros;
+//   * embed_join_kernel adds the parts of each run that crossed, in the chunks' order.
 #include "pf_elem.h"
 
 namespace {
@@ -53,11 +52,14 @@ __global__ __launch_bounds__(256) void embed_kernel(const I* __restrict__ t, con
 }
 
 // ------------------------------------------------------------------------------ sorting
-// One pass of a stable least-significant-digit radix sort: at most SORT_BLOCKS workgroups, each with
-// a contiguous part of the list.  A pass is two launches (counts per workgroup and digit, then the
-// moves): every workgroup of the second adds up the others' counts itself, which at <= 512 digits
-// x 256 workgroups (512 KB from L2) costs less than a third launch.
-constexpr int SORT_BLOCKS = 256, SORT_TILE = 1024, SORT_BITS = 9;
+// Stable least-significant-digit radix sort of (token, position), digits of at most 9 bits.
+//   * up to SORT_SMALL tokens: one workgroup, all passes in LDS, one launch;
+//   * else each pass is a launch that counts the digits per workgroup (at most 2^17 / digits
+//     workgroups, each with a contiguous part of the list), one that turns the counts into first places,
+//     and one that moves.
+// A wave ranks 64 tokens at a time: the lanes with its digit come from one ballot per bit, and the
+// digit's counter of the wave is read by all of them and raised by the first.
+constexpr int SORT_TILE = 1024, SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_SMALL = 4096;
 
 struct SortPart {
   long n, per;    // tokens, and tokens per workgroup (a multiple of SORT_TILE)
@@ -76,10 +78,109 @@ PF_DEV uint32_t sort_key(const void* src, long i, long V) {
   }
 }
 
+// Rank of this lane's token (`in`: there is one) among those of digit d that the wave has seen since its
+// `counts` were cleared, and the counts with these 64 added.
+PF_DEV uint32_t wave_rank(uint32_t* counts, uint32_t d, int bits, bool in, int lane) {
+  uint64_t same = __ballot(in);   // the lanes with this digit
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t ones = __ballot((d >> b) & 1);
+    same &= (d >> b) & 1 ? ones : ~ones;
+  }
+  const int lower = __popcll(same & ((1ull << lane) - 1));
+  uint32_t seen = 0;
+  if (in) seen = counts[d];
+  // the wave's LDS accesses run in order; the fences keep the compiler to it: every lane has read
+  // before the first one adds, and the next 64 tokens read what was added
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (in && lower == 0) counts[d] = seen + (uint32_t)__popcll(same);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return seen + lower;
+}
+
+// Inclusive sum over the lanes up to this one.
+PF_DEV uint32_t wave_scan(uint32_t x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    x += lane >= o ? y : 0;
+  }
+  return x;
+}
+
+constexpr int SMALL_WAVES = 16;
+constexpr size_t SMALL_LDS = 4 * SORT_SMALL * 4 + SMALL_WAVES * SORT_BINS * 4 + 64;
+
+template <typename I>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void sort_small_kernel(const void* __restrict__ tokens, uint32_t* __restrict__ keys_out,
+                                                                      uint32_t* __restrict__ pos_out, SortPart p, int passes) {
+  extern __shared__ __align__(16) char smem[];
+  uint32_t* const keys = reinterpret_cast<uint32_t*>(smem);      // [2][SORT_SMALL]
+  uint32_t* const pos = keys + 2 * SORT_SMALL;                   // [2][SORT_SMALL]
+  uint32_t* const counts = pos + 2 * SORT_SMALL;                 // [SMALL_WAVES][SORT_BINS]
+  uint32_t* const sums = counts + SMALL_WAVES * SORT_BINS;       // [SMALL_WAVES]
+  const int n = (int)p.n, bins = 1 << p.bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int NT = 64 * SMALL_WAVES, ITEMS = SORT_SMALL / NT;
+  for (int i = tid; i < n; i += NT) {
+    keys[i] = sort_key<I, true>(tokens, i, p.V);
+    pos[i] = i;
+  }
+  // a wave's share of the list, whole 64s
+  const int share = (n + 64 * SMALL_WAVES - 1) / (64 * SMALL_WAVES) * 64;
+  for (int pass = 0; pass < passes; ++pass) {
+    const uint32_t *ki = keys + (pass & 1) * SORT_SMALL, *pi = pos + (pass & 1) * SORT_SMALL;
+    uint32_t *ko = keys + (1 - (pass & 1)) * SORT_SMALL, *po = pos + (1 - (pass & 1)) * SORT_SMALL;
+    for (int d = tid; d < SMALL_WAVES * SORT_BINS; d += NT) counts[d] = 0;
+    __syncthreads();
+    uint32_t key[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int i = wave * share + 64 * u + lane;
+      const bool in = 64 * u < share && i < n;
+      key[u] = in ? ki[i] : 0;
+      if (64 * u < share) rank[u] = wave_rank(counts + wave * SORT_BINS, (key[u] >> (pass * p.bits)) & (bins - 1), p.bits, in, lane);
+    }
+    __syncthreads();
+    // first places: the digits before, then the waves before
+    uint32_t total = 0;
+    if (tid < bins) {
+      for (int w = 0; w < SMALL_WAVES; ++w) total += counts[w * SORT_BINS + tid];
+    }
+    const uint32_t upto = wave_scan(total, lane);
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    uint32_t at = upto - total;
+    for (int w = 0; w < wave; ++w) at += sums[w];
+    if (tid < bins) {
+      for (int w = 0; w < SMALL_WAVES; ++w) {
+        const uint32_t c = counts[w * SORT_BINS + tid];
+        counts[w * SORT_BINS + tid] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int i = wave * share + 64 * u + lane;
+      if (64 * u < share && i < n) {
+        const uint32_t to = counts[wave * SORT_BINS + ((key[u] >> (pass * p.bits)) & (bins - 1))] + rank[u];
+        ko[to] = key[u];
+        po[to] = pi[i];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += NT) {
+    keys_out[i] = keys[(passes & 1) * SORT_SMALL + i];
+    pos_out[i] = pos[(passes & 1) * SORT_SMALL + i];
+  }
+}
+
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(256) void sort_count_kernel(const void* __restrict__ keys, uint32_t* __restrict__ counts,
                                                          SortPart p) {
-  __shared__ uint32_t hist[1 << SORT_BITS];
+  __shared__ uint32_t hist[SORT_BINS];
   const int bins = 1 << p.bits;
   for (int d = threadIdx.x; d < bins; d += 256) hist[d] = 0;
   __syncthreads();
@@ -87,46 +188,50 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const void* __restrict_
   for (long i = (long)blockIdx.x * p.per + threadIdx.x; i < i1; i += 256)
     atomicAdd(&hist[(sort_key<I, FIRST>(keys, i, p.V) >> p.shift) & (bins - 1)], 1u);
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += 256) counts[(long)blockIdx.x * bins + d] = hist[d];
+  for (int d = threadIdx.x; d < bins; d += 256) counts[(long)d * gridDim.x + blockIdx.x] = hist[d];
+}
+
+// counts [digit][workgroup]: a wave per digit replaces them by the sums of the workgroups before, and
+// leaves the digit's total behind them (totals[digit]).
+__global__ __launch_bounds__(64) void sort_scan_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int blocks) {
+  uint32_t* const c = counts + (long)blockIdx.x * blocks;
+  const int lane = threadIdx.x;
+  uint32_t before = 0;
+  for (int b0 = 0; b0 < blocks; b0 += 64) {
+    const int b = b0 + lane;
+    const uint32_t x = b < blocks ? c[b] : 0, upto = wave_scan(x, lane);
+    if (b < blocks) c[b] = before + upto - x;
+    before += __shfl(upto, 63);
+  }
+  if (lane == 0) totals[blockIdx.x] = before;
 }
 
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(256) void sort_move_kernel(const void* __restrict__ keys, const uint32_t* __restrict__ pos,
-                                                        const uint32_t* __restrict__ counts, uint32_t* __restrict__ keys_out,
-                                                        uint32_t* __restrict__ pos_out, SortPart p) {
-  constexpr int BINS = 1 << SORT_BITS, ITEMS = SORT_TILE / 256;
-  __shared__ uint32_t base[BINS];        // where the next token of a digit goes
-  __shared__ uint32_t wave_n[4][BINS];   // tokens of a digit per wave of this tile, then their first place
-  __shared__ uint32_t scan[256];
+                                                        const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
+                                                        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, SortPart p) {
+  constexpr int ITEMS = SORT_TILE / 256;
+  __shared__ uint32_t base[SORT_BINS];        // where the next token of a digit goes
+  __shared__ uint32_t wave_n[4][SORT_BINS];   // tokens of a digit per wave of this tile, then their first place
+  __shared__ uint32_t sums[4];
   const int bins = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // totals per digit, and this workgroup's share before it
-  uint32_t before[2] = {0, 0}, total[2] = {0, 0};
+  uint32_t total[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) total[k] = 2 * (int)threadIdx.x + k < bins ? totals[2 * threadIdx.x + k] : 0;
+  const uint32_t upto = wave_scan(total[0] + total[1], lane);
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  uint32_t first = upto - total[0] - total[1];
+  for (int w = 0; w < wave; ++w) first += sums[w];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int d = 2 * threadIdx.x + k;
-    if (d < bins) {
-#pragma unroll 8
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const uint32_t c = counts[(long)b * bins + d];
-        total[k] += c;
-        before[k] += b < (int)blockIdx.x ? c : 0;
-      }
-    }
+    if (d < bins) base[d] = first + counts[(long)d * gridDim.x + blockIdx.x];
+    first += total[k];
   }
-  scan[threadIdx.x] = total[0] + total[1];
-  __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {
-    const uint32_t v = threadIdx.x >= (unsigned)o ? scan[threadIdx.x - o] : 0;
-    __syncthreads();
-    scan[threadIdx.x] += v;
-    __syncthreads();
-  }
-  const uint32_t first = scan[threadIdx.x] - total[0] - total[1];
-  if (2 * (int)threadIdx.x < bins) base[2 * threadIdx.x] = first + before[0];
-  if (2 * (int)threadIdx.x + 1 < bins) base[2 * threadIdx.x + 1] = first + total[0] + before[1];
   const long begin = (long)blockIdx.x * p.per, end = min(p.n, begin + p.per);
   for (long t0 = begin; t0 < end; t0 += SORT_TILE) {
-    for (int d = threadIdx.x; d < 4 * BINS; d += 256) (&wave_n[0][0])[d] = 0;
+    for (int d = threadIdx.x; d < 4 * SORT_BINS; d += 256) (&wave_n[0][0])[d] = 0;
     __syncthreads();
     // wave w ranks tokens t0 + 256 w .. + 255 in order, 64 at a time
     uint32_t key[ITEMS], at[ITEMS], rank[ITEMS];
@@ -137,26 +242,8 @@ __global__ __launch_bounds__(256) void sort_move_kernel(const void* __restrict__
       at[u] = i < end ? (FIRST ? (uint32_t)i : pos[i]) : 0;
     }
 #pragma unroll
-    for (int u = 0; u < ITEMS; ++u) {
-      const bool in = t0 + 256 * wave + 64 * u + lane < end;
-      const uint32_t d = (key[u] >> p.shift) & (bins - 1);
-      uint64_t same = __ballot(in);   // the lanes with this digit
-      for (int b = 0; b < p.bits; ++b) {
-        const uint64_t ones = __ballot((d >> b) & 1);
-        same &= (d >> b) & 1 ? ones : ~ones;
-      }
-      const int lower = __popcll(same & ((1ull << lane) - 1));
-      uint32_t seen = 0;
-      if (in) seen = wave_n[wave][d];
-      // the wave's LDS accesses run in order; the fences keep the compiler to it: every lane has read
-      // before the first one adds, and the next 64 tokens read what was added
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (in && lower == 0) wave_n[wave][d] = seen + (uint32_t)__popcll(same);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      rank[u] = seen + lower;
-    }
+    for (int u = 0; u < ITEMS; ++u)
+      rank[u] = wave_rank(wave_n[wave], (key[u] >> p.shift) & (bins - 1), p.bits, t0 + 256 * wave + 64 * u + lane < end, lane);
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += 256) {
       uint32_t s = base[d];
@@ -194,140 +281,210 @@ PF_DEV long lower_bound(const uint32_t* __restrict__ keys, long n, uint32_t v) {
 }
 
 // ------------------------------------------------------------------------------ sums
-constexpr int GRAD_ROWS = 128;   // most table rows of a workgroup of part 1
-
 struct GradPart {
   long n, V, C;
+  int ch;                // CH, a multiple of 8
   long chunks;           // of CH sorted tokens
-  int ch;                // CH
-  int rows;              // table rows per workgroup of part 1
+  long chunk_blocks;     // workgroups of part 1
+  int rows;              // table rows per workgroup of part 2, groups of lanes x a whole number
   long row_blocks;
   float scale;
   int tpr_log2;          // lanes per row, a power of two <= 256
 };
 
-// a += rows g[pos[i]], i = s, s + by, .. < e, at channels c .. c + N in fp32, U of them in flight.
-template <typename T, int N>
-PF_DEV void sum_rows(const T* __restrict__ g, const uint32_t* __restrict__ pos, long C, long s, long e, int by, long c,
-                     float (&a)[N]) {
-  constexpr int U = 8;
-  for (long i0 = s; i0 < e; i0 += (long)by * U) {
-    float v[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long i = i0 + (long)u * by;
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[u][k] = 0.f;
-      if (i < e) load_elems<T, N>(g + (long)pos[i] * C + c, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int k = 0; k < N; ++k) a[k] += v[u][k];
-  }
-}
+constexpr int GRAD_ROWS = 128;   // most table rows of a workgroup of part 2
 
 template <typename T, int N>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const T* __restrict__ g, const uint32_t* __restrict__ keys,
                                                          const uint32_t* __restrict__ pos, T* __restrict__ dw,
-                                                         float* __restrict__ parts, int* __restrict__ long_end, GradPart p) {
-  __shared__ float part[N * 256];
-  __shared__ long bound[GRAD_ROWS + 1];
+                                                         float* __restrict__ parts, GradPart p) {
+  __shared__ long bound[2 * GRAD_ROWS];
   const int lane = threadIdx.x & ((1 << p.tpr_log2) - 1), group = threadIdx.x >> p.tpr_log2, groups = 256 >> p.tpr_log2;
   const long step = (long)N << p.tpr_log2;
-  if ((long)blockIdx.x >= p.chunks) {   // part 1: table rows v0 .. v0 + rows
-    const long v0 = ((long)blockIdx.x - p.chunks) * p.rows;
-    const int rows = (int)min((long)p.rows, p.V - v0);
-    if ((int)threadIdx.x <= rows) bound[threadIdx.x] = lower_bound(keys, p.n, (uint32_t)(v0 + threadIdx.x));
+  if ((long)blockIdx.x >= p.chunk_blocks) {
+    // part 2: zeros for the rows that no token names.  Neighbouring workgroups take neighbouring rows (a
+    // workgroup on consecutive rows of its own leaves the chip writing far-apart pieces at a time).
+    const long k = (long)blockIdx.x - p.chunk_blocks;
+    auto row_of = [&](int r) __attribute__((always_inline)) {
+      return ((long)(r / groups) * p.row_blocks + k) * groups + r % groups;
+    };
+    if ((int)threadIdx.x < 2 * p.rows) {
+      const long v = row_of(threadIdx.x >> 1);
+      bound[threadIdx.x] = v < p.V ? lower_bound(keys, p.n, (uint32_t)(v + (threadIdx.x & 1))) : threadIdx.x & 1;
+    }
     __syncthreads();
-    for (int r = group; r < rows; r += groups) {
-      const long s = bound[r], e = bound[r + 1];
-      if (e - s > p.ch) continue;
-      for (long c = (long)lane * N; c < p.C; c += step) {
-        float a[N];
+    float zero[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) a[i] = 0.f;
-        sum_rows<T, N>(g, pos, p.C, s, e, 1, c, a);
-#pragma unroll
-        for (int i = 0; i < N; ++i) a[i] *= p.scale;
-        store_elems<T, N>(dw + (v0 + r) * p.C + c, a);
-      }
+    for (int i = 0; i < N; ++i) zero[i] = 0.f;
+    for (int r = group; r < p.rows; r += groups) {
+      if (bound[2 * r] != bound[2 * r + 1]) continue;
+      T* const to = dw + row_of(r) * p.C;
+      for (long c = (long)lane * N; c < p.C; c += step) store_elems<T, N>(to + c, zero);
     }
     return;
   }
-  // part 2: what long runs have in this chunk
-  const long i0 = (long)blockIdx.x * p.ch, i1 = min(p.n, i0 + p.ch);
-  if (threadIdx.x < 4) {   // the runs of the first and of the last token
-    const uint32_t v = keys[threadIdx.x < 2 ? i0 : i1 - 1];
-    bound[threadIdx.x] = lower_bound(keys, p.n, v + (threadIdx.x & 1));
-  }
-  __syncthreads();
-  const long s0 = bound[0], e0 = bound[1], s1 = bound[2], e1 = bound[3];
-  const bool first = e0 - s0 > p.ch && keys[i0] < (uint32_t)p.V;
-  const bool last = s1 > i0 && e1 - s1 > p.ch && keys[i1 - 1] < (uint32_t)p.V;
-  // a long run that begins in this chunk: the join's work
-  if (threadIdx.x == 0) long_end[blockIdx.x] = last ? (int)e1 : first && s0 == i0 ? (int)e0 : 0;
-  for (int w = 0; w < 2; ++w) {
-    if (!(w ? last : first)) continue;
-    const long s = w ? s1 : i0, e = w ? i1 : min(i1, e0);
-    // the groups take the rows in turn, and their sums are joined in the groups' order
-    for (long c0 = 0; c0 < p.C; c0 += step) {
-      const long c = c0 + (long)lane * N;
-      float a[N];
+  // part 1: a group of lanes streams the CH tokens of a chunk in their sorted order, U rows in flight, and
+  // writes a sum where the token changes
+  constexpr int U = 8;
+  const long chunk = (long)blockIdx.x * groups + group;
+  if (chunk >= p.chunks) return;
+  const long i0 = chunk * p.ch, i1 = min(p.n, i0 + p.ch);
+  const uint32_t none = (uint32_t)p.V;
+  const bool goes_on = i0 > 0 && keys[i0 - 1] == keys[i0];   // its first run began before
+  const bool reaches = i1 < p.n && keys[i1] == keys[i1 - 1]; // its last run goes on behind
+  float* const part0 = parts + 2 * chunk * p.C;
+  for (long c = (long)lane * N; c < p.C; c += step) {
+    uint32_t cur = keys[i0];
+    if (cur >= none) return;   // sorted behind all others: nothing here, or later
+    bool first = goes_on;
+    float a[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) a[i] = 0.f;
-      if (c < p.C) sum_rows<T, N>(g, pos, p.C, s + group, e, groups, c, a);
-      if (groups > 1) {
+    for (int k = 0; k < N; ++k) a[k] = 0.f;
+    auto flush = [&](bool part, float* to) __attribute__((always_inline)) {
+      if (part) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) part[i * 256 + threadIdx.x] = a[i];
-        for (int o = groups >> 1; o >= 1; o >>= 1) {
-          __syncthreads();
-          if (group < o) {
+        for (int k = 0; k < N; ++k) to[c + k] = a[k];
+      } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              a[i] += part[i * 256 + threadIdx.x + (o << p.tpr_log2)];
-              part[i * 256 + threadIdx.x] = a[i];
-            }
-          }
-        }
-        __syncthreads();
+        for (int k = 0; k < N; ++k) a[k] *= p.scale;
+        store_elems<T, N>(dw + (long)cur * p.C + c, a);
       }
-      if (group == 0 && c < p.C) {
+    };
+    uint32_t key[U], at[U];
 #pragma unroll
-        for (int i = 0; i < N; ++i) parts[(2l * blockIdx.x + w) * p.C + c + i] = a[i];
+    for (int u = 0; u < U; ++u) {
+      const long i = min(i0 + u, i1 - 1);
+      key[u] = keys[i], at[u] = pos[i];
+    }
+    for (long i = i0; i < i1 && key[0] < none; i += U) {
+      float v[U][N];
+      uint32_t now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[u][k] = 0.f;
+        now[u] = key[u];
+        if (i + u < i1 && key[u] < none) load_elems<T, N>(g + (long)at[u] * p.C + c, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {   // the next tokens, behind the rows' loads
+        const long j = min(i + U + u, i1 - 1);
+        key[u] = keys[j], at[u] = pos[j];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (now[u] != cur) {
+          if (cur < none) flush(first, part0);
+          first = false;
+          cur = now[u];
+#pragma unroll
+          for (int k = 0; k < N; ++k) a[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) a[k] += v[u][k];
       }
     }
+    if (cur < none) flush(first || reaches, first ? part0 : part0 + p.C);
   }
 }
 
-// The parts of the long run that begins in chunk blockIdx.x, if one does: its first part, then the
-// first-token parts of the chunks up to its end.  One channel a lane.
-template <typename T>
-__global__ __launch_bounds__(256) void embed_join_kernel(const float* __restrict__ parts, const uint32_t* __restrict__ keys,
-                                                         const int* __restrict__ long_end, T* __restrict__ dw, GradPart p) {
-  __shared__ float part[256];
-  const long c0 = blockIdx.x, e = long_end[c0];
-  if (e == 0) return;
-  const uint32_t v = keys[e - 1];
-  const long c1 = (e - 1) / p.ch;
-  const bool whole = keys[c0 * p.ch] == v;   // the run holds the chunk's first token too
-  const int lane = threadIdx.x & ((1 << p.tpr_log2) - 1), group = threadIdx.x >> p.tpr_log2, groups = 256 >> p.tpr_log2;
-  for (long c = (long)blockIdx.y << p.tpr_log2; c < p.C; c += (long)gridDim.y << p.tpr_log2) {
-    const bool in = c + lane < p.C;
-    float a = 0.f;
-    if (in) {
-#pragma unroll 8
-      for (long k = c0 + group; k <= c1; k += groups) a += parts[(2 * k + (k == c0 && !whole)) * p.C + c + lane];
+// The runs that begin in a workgroup's JOIN chunks and go on behind their chunk: the run's own part, then
+// the following chunks' first parts.  A wave adds a run of up to JOIN_SHORT parts by itself; a longer one
+// is split over the waves.  N channels a lane, blockIdx.y counts blocks of 64 N channels.
+constexpr int JOIN = 32, JOIN_WAVES = 8, JOIN_SHORT = 32;
+
+template <typename T, int N>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join_kernel(const float* __restrict__ parts, const uint32_t* __restrict__ keys,
+                                                                     T* __restrict__ dw, GradPart p) {
+  __shared__ float part[JOIN_WAVES][N][64];
+  __shared__ long last[JOIN];       // last chunk of the run that begins in a chunk (0: none does)
+  __shared__ uint32_t token[JOIN];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long c00 = (long)blockIdx.x * JOIN;
+  if (threadIdx.x < JOIN) {
+    const long c0 = c00 + threadIdx.x, i0 = c0 * p.ch, i1 = i0 + p.ch;
+    long end = 0;
+    if (i1 < p.n) {
+      const uint32_t v = keys[i1 - 1];
+      if (v < (uint32_t)p.V && keys[i1] == v && !(i0 > 0 && keys[i0] == v && keys[i0 - 1] == v)) {
+        end = c0 + 1;
+        token[threadIdx.x] = v;
+      }
     }
-    if (groups > 1) {
-      part[threadIdx.x] = a;
-      for (int o = groups >> 1; o >= 1; o >>= 1) {
-        __syncthreads();
-        if (group < o) part[threadIdx.x] = a = a + part[threadIdx.x + (o << p.tpr_log2)];
+    last[threadIdx.x] = end;
+  }
+  __syncthreads();
+  // how far the runs go: 64 chunk beginnings at a time, 64 times as far apart while all of them match
+  for (int j = wave; j < JOIN; j += JOIN_WAVES) {
+    long lo = last[j];   // chunk lo begins with the token
+    if (lo == 0) continue;
+    const uint32_t v = token[j];
+    bool grow = true;
+    for (long hop = 1; hop >= 1;) {
+      const long k = lo + hop * (lane + 1);
+      const int match = __popcll(__ballot(k < p.chunks && keys[k < p.chunks ? k * p.ch : 0] == v));
+      lo += hop * match;
+      grow = grow && match == 64;
+      hop = grow ? hop * 64 : hop / 64;
+    }
+    if (lane == 0) last[j] = lo;
+  }
+  __syncthreads();
+  // lanes of a wave beyond a row's take further parts of the same run
+  const int tpr = 1 << p.tpr_log2, sub = lane >> p.tpr_log2, subs = 64 >> p.tpr_log2;
+  auto add = [&](long c0, long from, long to, int by, long c, float (&a)[N]) __attribute__((always_inline)) {
+    constexpr int U = 8;
+    for (long k0 = from; k0 <= to; k0 += (long)by * U) {
+      float x[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long k = k0 + (long)u * by;
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[u][e] = 0.f;
+        if (k <= to) load_elems<float, N>(parts + (2 * k + (k == c0)) * p.C + c, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) a[e] += x[u][e];
+    }
+  };
+  for (long cb = (long)blockIdx.y * tpr * N; cb < p.C; cb += (long)gridDim.y * tpr * N) {
+    const long c = cb + (lane & (tpr - 1)) * N;
+    const bool in = c < p.C;
+    for (int j = wave; j < JOIN; j += JOIN_WAVES) {
+      const long c0 = c00 + j, c1 = last[j];
+      if (c1 == 0 || c1 - c0 >= JOIN_SHORT || !in || sub) continue;
+      float a[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) a[e] = 0.f;
+      add(c0, c0, c1, 1, c, a);
+      T* const to = dw + (long)token[j] * p.C + c;
+#pragma unroll
+      for (int e = 0; e < N; ++e) to[e] = (T)(a[e] * p.scale);
+    }
+    for (int j = 0; j < JOIN; ++j) {
+      const long c0 = c00 + j, c1 = last[j];
+      if (c1 == 0 || c1 - c0 < JOIN_SHORT) continue;
+      float a[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) a[e] = 0.f;
+      if (in) add(c0, c0 + wave * subs + sub, c1, JOIN_WAVES * subs, c, a);
+#pragma unroll
+      for (int e = 0; e < N; ++e) part[wave][e][lane] = a[e];
+      __syncthreads();
+      if (wave == 0 && sub == 0 && in) {
+        T* const to = dw + (long)token[j] * p.C + c;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          float s = 0.f;
+          for (int w = 0; w < JOIN_WAVES; ++w)
+            for (int u = 0; u < subs; ++u) s += part[w][e][lane + u * tpr];
+          to[e] = (T)(s * p.scale);
+        }
       }
       __syncthreads();
     }
-    if (group == 0 && in) dw[(long)v * p.C + c + lane] = (T)(a * p.scale);
   }
 }
 
@@ -341,7 +498,7 @@ int log2_at_least(long n) {
 struct GradLayout {
   int passes, bits, ch;
   long per, blocks, chunks;
-  size_t keys, pos, counts, ends, parts, bytes;
+  size_t keys, pos, counts, totals, parts, bytes;
 };
 
 GradLayout grad_layout(long n, long V, long C) {
@@ -350,17 +507,22 @@ GradLayout grad_layout(long n, long V, long C) {
   l.passes = (all + SORT_BITS - 1) / SORT_BITS;
   l.bits = (all + l.passes - 1) / l.passes;
   const long tiles = n > 0 ? (n + SORT_TILE - 1) / SORT_TILE : 1;
-  l.per = (tiles + SORT_BLOCKS - 1) / SORT_BLOCKS * SORT_TILE;
+  const long most = (1l << 17) >> l.bits;   // workgroups: their counts stay within 512 KB
+  l.per = (tiles + most - 1) / most * SORT_TILE;
   l.blocks = (n + l.per - 1) / l.per;
-  l.ch = n <= (1l << 17) ? 64 : 256;
+  // chunks of 32 tokens while that gives the chip no more than 2^18 lanes, longer ones (fewer crossed
+  // borders) behind that; C / 4 lanes a row at most
+  const int lanes = C >= 1024 ? 256 : 1 << log2_at_least((C + 3) / 4);
+  l.ch = 32;
+  while (l.ch < 256 && n / l.ch * lanes > (1l << 18)) l.ch *= 2;
   l.chunks = (n + l.ch - 1) / l.ch;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
   const size_t list = up((size_t)n * 4);
   l.keys = 0;
   l.pos = 2 * list;
   l.counts = 4 * list;
-  l.ends = l.counts + up(((size_t)l.blocks << l.bits) * 4);
-  l.parts = l.ends + up((size_t)l.chunks * 4);
+  l.totals = l.counts + up(((size_t)l.blocks << l.bits) * 4);
+  l.parts = l.totals + up((size_t)4 << l.bits);
   l.bytes = l.parts + up((size_t)l.chunks * 2 * C * 4);
   return l;
 }
@@ -402,24 +564,30 @@ int embed_type(const void* t, int index64, const void* w, long ldw, void* out, l
 
 template <typename I>
 int sort_tokens(const void* index, char* ws, const GradLayout& l, long n, long V, hipStream_t st, int* result) {
-  uint32_t *keys[2], *pos[2], *counts = (uint32_t*)(ws + l.counts);
+  uint32_t *keys[2], *pos[2], *counts = (uint32_t*)(ws + l.counts), *totals = (uint32_t*)(ws + l.totals);
   const size_t list = (l.pos - l.keys) / 2;
   for (int k = 0; k < 2; ++k) {
     keys[k] = (uint32_t*)(ws + l.keys + k * list);
     pos[k] = (uint32_t*)(ws + l.pos + k * list);
   }
+  if (n <= SORT_SMALL) {
+    if (int rc = pf_reserve_lds((const void*)sort_small_kernel<I>, SMALL_LDS, "sort_small_kernel")) return rc;
+    sort_small_kernel<I><<<1, 64 * SMALL_WAVES, SMALL_LDS, st>>>(index, keys[0], pos[0], SortPart{n, l.per, V, 0, l.bits}, l.passes);
+    PF_CHECK_LAUNCH("sort_small_kernel");
+    *result = 0;
+    return PF_OK;
+  }
   for (int pass = 0; pass < l.passes; ++pass) {
     const SortPart p{n, l.per, V, pass * l.bits, l.bits};
     const int to = pass & 1, from = 1 - to;
-    if (pass == 0) {
-      sort_count_kernel<I, true><<<(unsigned)l.blocks, 256, 0, st>>>(index, counts, p);
-      PF_CHECK_LAUNCH("sort_count_kernel");
-      sort_move_kernel<I, true><<<(unsigned)l.blocks, 256, 0, st>>>(index, nullptr, counts, keys[to], pos[to], p);
-    } else {
-      sort_count_kernel<I, false><<<(unsigned)l.blocks, 256, 0, st>>>(keys[from], counts, p);
-      PF_CHECK_LAUNCH("sort_count_kernel");
-      sort_move_kernel<I, false><<<(unsigned)l.blocks, 256, 0, st>>>(keys[from], pos[from], counts, keys[to], pos[to], p);
-    }
+    const unsigned grid = (unsigned)l.blocks;
+    if (pass == 0) sort_count_kernel<I, true><<<grid, 256, 0, st>>>(index, counts, p);
+    else sort_count_kernel<I, false><<<grid, 256, 0, st>>>(keys[from], counts, p);
+    PF_CHECK_LAUNCH("sort_count_kernel");
+    sort_scan_kernel<<<1u << l.bits, 64, 0, st>>>(counts, totals, (int)l.blocks);
+    PF_CHECK_LAUNCH("sort_scan_kernel");
+    if (pass == 0) sort_move_kernel<I, true><<<grid, 256, 0, st>>>(index, nullptr, counts, totals, keys[to], pos[to], p);
+    else sort_move_kernel<I, false><<<grid, 256, 0, st>>>(keys[from], pos[from], counts, totals, keys[to], pos[to], p);
     PF_CHECK_LAUNCH("sort_move_kernel");
   }
   *result = (l.passes - 1) & 1;
@@ -429,20 +597,22 @@ int sort_tokens(const void* index, char* ws, const GradLayout& l, long n, long V
 template <typename T, int N>
 int grad_sums(const T* g, const uint32_t* keys, const uint32_t* pos, T* dw, char* ws, const GradLayout& l, long n, long V,
               long C, float scale, hipStream_t st) {
-  const int units = (int)((C + N - 1) / N), tpr_log2 = units >= 256 ? 8 : log2_at_least(units);
-  // a row for each group of lanes at least; more where eight workgroups per CU remain
-  const long groups = 256 >> tpr_log2, share = V / 2048 < 64 ? V / 2048 : 64;
-  const int rows = (int)(groups > GRAD_ROWS ? GRAD_ROWS : share < groups ? groups : share);
-  GradPart p{n, V, C, l.chunks, l.ch, rows, (V + rows - 1) / rows, scale, tpr_log2};
+  const int units = (int)((C + N - 1) / N), tpr_log2 = units >= 256 ? 8 : units <= 2 ? 1 : log2_at_least(units);
+  const long groups = 256 >> tpr_log2;
+  // part 2: a row for each group of lanes at least; up to 64 where four workgroups per CU remain
+  long rows = V / 1024 < 64 ? V / 1024 / groups * groups : 64 / groups * groups;
+  if (rows < groups) rows = groups;
+  GradPart p{n, V, C, l.ch, l.chunks, (l.chunks + groups - 1) / groups, (int)rows, (V + rows - 1) / rows, scale, tpr_log2};
   float* parts = (float*)(ws + l.parts);
-  int* ends = (int*)(ws + l.ends);
-  if ((p.chunks + p.row_blocks) >> 24) return pf_fail(PF_E_INVALID, "pf_embedding_grad: too many rows (n=%ld V=%ld C=%ld)", n, V, C);
-  embed_grad_kernel<T, N><<<(unsigned)(p.chunks + p.row_blocks), 256, 0, st>>>(g, keys, pos, dw, parts, ends, p);
+  if ((p.chunk_blocks + p.row_blocks) >> 24)
+    return pf_fail(PF_E_INVALID, "pf_embedding_grad: too many rows (n=%ld V=%ld C=%ld)", n, V, C);
+  embed_grad_kernel<T, N><<<(unsigned)(p.chunk_blocks + p.row_blocks), 256, 0, st>>>(g, keys, pos, dw, parts, p);
   PF_CHECK_LAUNCH("embed_grad_kernel");
-  if (l.chunks == 0 || n <= l.ch) return PF_OK;   // no run can be longer than a chunk
-  p.tpr_log2 = C >= 64 ? 6 : log2_at_least(C);
-  const long cols = (C + (1l << p.tpr_log2) - 1) >> p.tpr_log2;
-  embed_join_kernel<T><<<dim3((unsigned)l.chunks, (unsigned)(cols < 32 ? cols : 32)), 256, 0, st>>>(parts, keys, ends, dw, p);
+  if (l.chunks <= 1) return PF_OK;   // no run crosses a border
+  constexpr int J = N > 1 ? 4 : 1;
+  p.tpr_log2 = C >= 64 * J ? 6 : log2_at_least((C + J - 1) / J);
+  const long cols = (C + 64 * J - 1) / (64 * J), blocks = (l.chunks + JOIN - 1) / JOIN;
+  embed_join_kernel<T, J><<<dim3((unsigned)blocks, (unsigned)(cols < 64 ? cols : 64)), 64 * JOIN_WAVES, 0, st>>>(parts, keys, dw, p);
   PF_CHECK_LAUNCH("embed_join_kernel");
   return PF_OK;
 }
