@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const T* __restrict__ g
 // The runs that begin in a workgroup's JOIN chunks and go on behind their chunk: the run's own part, then
 // the following chunks' first parts.  A wave adds a run of up to JOIN_SHORT parts by itself; a longer one
 // is split over the waves.  N channels a lane, blockIdx.y counts blocks of 64 N channels.
-constexpr int JOIN = 32, JOIN_WAVES = 8, JOIN_SHORT = 32;
+constexpr int JOIN = 8, JOIN_WAVES = 8, JOIN_SHORT = 32;
 
 template <typename T, int N>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join_kernel(const float* __restrict__ parts, const uint32_t* __restrict__ keys,
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join_kernel(const float
     }
     last[threadIdx.x] = end;
   }
-  __syncthreads();
+  if (!__syncthreads_or(threadIdx.x < JOIN && last[threadIdx.x])) return;
   // how far the runs go: 64 chunk beginnings at a time, 64 times as far apart while all of them match
   for (int j = wave; j < JOIN; j += JOIN_WAVES) {
     long lo = last[j];   // chunk lo begins with the token
@@ -470,6 +470,10 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join_kernel(const float
 #pragma unroll
       for (int e = 0; e < N; ++e) a[e] = 0.f;
       if (in) add(c0, c0 + wave * subs + sub, c1, JOIN_WAVES * subs, c, a);
+      for (int o = tpr; o < 64; o <<= 1) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) a[e] += __shfl_xor(a[e], o);
+      }
 #pragma unroll
       for (int e = 0; e < N; ++e) part[wave][e][lane] = a[e];
       __syncthreads();
@@ -478,8 +482,8 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join_kernel(const float
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           float s = 0.f;
-          for (int w = 0; w < JOIN_WAVES; ++w)
-            for (int u = 0; u < subs; ++u) s += part[w][e][lane + u * tpr];
+#pragma unroll
+          for (int w = 0; w < JOIN_WAVES; ++w) s += part[w][e][lane];
           to[e] = (T)(s * p.scale);
         }
       }
