@@ -640,3 +640,11 @@ def test_cross_attention_launchers_in_two_graphs(gpu):
         for _, c, do, outs, _, _ in graphs:
             o, grads = run_cross(c, do, gpu)
             assert all(torch.equal(x, y) for x, y in zip(outs, (o, grads["dq"], grads["dk"], grads["dv"], grads["dbias"])))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hide", [None, "both"])
+def test_cross_attention_many_heads(gpu, dtype, hide):
+    """512 workgroups of 256 rows and more: two row tiles per wave."""
+    c, do = inputs(16, dtype, 64, 70, 150, 8, 8, 48, None, hide)
+    check_cross(c, do, gpu)

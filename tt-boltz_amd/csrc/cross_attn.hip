@@ -64,19 +64,19 @@ XaParams params_of(const pf_cross_attn_args* a) {
   p.few = p.rows <= 32;
   p.splits = p.per = 1;
   const int longest = p.rows > p.Lk ? p.rows : p.Lk;
-  p.chunks = longest > 64 * 128 ? 64 : (longest + 127) / 128;
+  p.chunks = longest > 64 * 32 ? 64 : (longest + 31) / 32;
   return p;
 }
 
-// the split over key tiles of the forward and the dq kernel
-Split key_split(const XaParams& p) {
+// the split over key tiles of the forward and the dq kernel (an fp32 tile is worth several of 16 bits)
+Split key_split(const XaParams& p, int dtype) {
   const long rows = p.few ? 32 : 128, kt = p.few ? XA_KT_FEW : XA_KT;
-  return split_of((p.rows + rows - 1) / rows * p.B * p.Hk, (p.Lk + kt - 1) / kt, p.few ? 1 : 4);
+  return split_of((p.rows + rows - 1) / rows * p.B * p.Hk, (p.Lk + kt - 1) / kt, p.few ? 1 : dtype == PF_FP32 ? 2 : 4);
 }
 // the split over row tiles of the dk, dv kernel
 Split row_split(const XaParams& p, int dtype) {
   const int rt = xa_rt(p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128, dtype == PF_FP32);
-  return split_of((long)(p.Lk + XA_KEYS - 1) / XA_KEYS * p.B * p.Hk, ((long)p.Lq + rt - 1) / rt * p.G, 256 / rt);
+  return split_of((long)(p.Lk + XA_KEYS - 1) / XA_KEYS * p.B * p.Hk, ((long)p.Lq + rt - 1) / rt * p.G, dtype == PF_FP32 ? 2 : 256 / rt);
 }
 
 long fwd_part_bytes(const XaParams& p, const Split& s) {
@@ -92,7 +92,7 @@ BwdLayout bwd_layout(const pf_cross_attn_args* a, const XaParams& p) {
   l.ds = l.amax + up256((long)p.B * p.Hk * p.chunks * 8);
   const bool own = a->dbias_B > 0 && !(a->bias_dtype == PF_FP32 && a->dbias_B == a->B && a->dbias_H == a->H);
   l.part = l.ds + (own ? up256((long)p.B * p.H * p.Lq * p.Lk * 4) : 0);
-  const Split ks = key_split(p), rs = row_split(p, a->dtype);
+  const Split ks = key_split(p, a->dtype), rs = row_split(p, a->dtype);
   const long dq = ks.splits > 1 ? (long)ks.splits * p.B * p.Lq * p.H * p.D * 4 : 0;
   const long dkv = rs.splits > 1 ? 2l * rs.splits * p.B * p.Lk * p.Hk * p.D * 4 : 0;
   l.bytes = l.part + (dq > dkv ? dq : dkv);
@@ -137,7 +137,7 @@ int dbias_launch(const float* ds, void* out, const pf_cross_attn_args* a, hipStr
 extern "C" size_t pf_cross_attn_workspace_size(const pf_cross_attn_args* a) {
   if (check(a, "pf_cross_attn_workspace_size")) return 0;
   const XaParams p = params_of(a);
-  return (size_t)fwd_part_bytes(p, key_split(p));
+  return (size_t)fwd_part_bytes(p, key_split(p, a->dtype));
 }
 
 extern "C" int pf_cross_attn_fwd(const pf_cross_attn_args* a) {
@@ -149,7 +149,7 @@ extern "C" int pf_cross_attn_fwd(const pf_cross_attn_args* a) {
   if (!pf_aligned16(a->o) || !pf_aligned16(a->o32)) return pf_fail(PF_E_INVALID, "%s: o must be 16-byte aligned", fn);
   XaParams p = params_of(a);
   if (!grid_fits(p)) return pf_fail(PF_E_INVALID, "%s: too large (B=%d Lq=%d Lk=%d H=%d)", fn, a->B, a->Lq, a->Lk, a->H);
-  const Split s = key_split(p);
+  const Split s = key_split(p, a->dtype);
   const size_t need = (size_t)fwd_part_bytes(p, s);
   if (need && (!a->workspace || a->workspace_bytes < need))
     return pf_fail(PF_E_INVALID, "%s: workspace too small (%zu < %zu bytes)", fn, a->workspace_bytes, need);
@@ -208,14 +208,14 @@ extern "C" int pf_cross_attn_bwd(const pf_cross_attn_args* a) {
     return rc;
   p.delta = delta;
   if (exact) {
-    const Split s = key_split(p);
+    const Split s = key_split(p, a->dtype);
     XaParams d = p;
     d.splits = s.splits, d.per = s.per;
     if (s.splits == 1) d.part = delta;
     if (int rc = t == PF_FP16 ? pf_xa_exact_delta_fp16(d, st) : pf_xa_exact_delta_bf16(d, st)) return rc;
   }
   if (a->dq) {
-    const Split s = key_split(p);
+    const Split s = key_split(p, a->dtype);
     XaParams d = p;
     d.splits = s.splits, d.per = s.per;
     const bool own = a->dbias && !(a->bias_dtype == PF_FP32 && a->dbias_B == a->B && a->dbias_H == a->H);

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
 template <typename T, int DP, bool BIAS, bool FEW>
 constexpr int dq_waves() {
   if (DP == 128) return FEW || __is_same(T, float) ? 1 : 2;
-  return __is_same(T, float) || DP == 64 ? 2 : BIAS || FEW ? 3 : 4;
+  return __is_same(T, float) || DP == 64 || BIAS ? 2 : FEW ? 3 : 4;
 }
 
 template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
@@ -137,9 +137,10 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
   const T* const vb = (const T*)p.v + b * p.vb + hk * p.vh;
 
   Stage<T, DP, KT> sk, sv;
-  auto load_tile = [&](int t) __attribute__((always_inline)) {
-    load_keys(sk, kb, p.kl, p.D, t, len, mask);
-    load_keys(sv, vb, p.vl, p.D, t, len, mask);
+  Seen<KT> now, next;
+  auto load_tile = [&](int t, const Seen<KT>& seen) __attribute__((always_inline)) {
+    load_keys(sk, kb, p.kl, p.D, t, seen);
+    load_keys(sv, vb, p.vl, p.D, t, seen);
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;
@@ -147,8 +148,17 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[0][dt] = zero16();
 
+  float bs[NSUB][16];
+  auto fetch_bias = [&](int t, int u) __attribute__((always_inline)) {
+    if constexpr (BIAS) load_bias16<T>(p, bias, t * KT + sub0 + 32 * u + 4 * h, row_ok, bs[u]);
+  };
   if (t0 < t1) {
-    load_tile(t0);
+    now.fetch(t0, len, mask);
+    next.fetch(t0 + 1, len, mask);
+    now.take();
+    load_tile(t0, now);
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) fetch_bias(t0, u);
     sk.store(ks0, KS);
     sv.store(ks0 + KT * KS, KS);
   }
@@ -156,22 +166,19 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
   for (int t = t0; t < t1; ++t) {
     const T* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
     const T* const vs = ks + KT * KS;
-    if (t + 1 < t1) load_tile(t + 1);
-    uint64_t word = ~0ull;
-    if (mask || (t + 1) * KT > len) {
-      const int key_l = t * KT + sub0 + (FEW ? n : lane);
-      word = __ballot(key_l < len && (!mask || mask[key_l]));
-    }
+    next.take();
+    if (t + 1 < t1) load_tile(t + 1, next);
+    Seen<KT> then;
+    then.fetch(t + 2, len, mask);
+    const uint64_t word = FEW ? now.part(wid) : now.w[0];
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
       const uint32_t word_u = (uint32_t)(word >> (FEW ? 0 : 32 * u));
-      if (!word_u && (DELTA || !p.ds)) continue;
-      const int key0 = t * KT + sub0 + 32 * u + 4 * h;
-      float bs[4][4];
-      if constexpr (BIAS) {
-#pragma unroll
-        for (int run = 0; run < 4; ++run) load_bias<T>(p, bias, key0 + 8 * run, row_ok, bs[run]);
+      if (!word_u && (DELTA || !p.ds)) {
+        if (t + 1 < t1) fetch_bias(t + 1, u);
+        continue;
       }
+      const int key0 = t * KT + sub0 + 32 * u + 4 * h;
       const int at = (sub0 + 32 * u + n) * KS + M::E * h;
       const f32x16 s = inner<T, DP>(ks + at, q, zero16());
       f32x16 y;
@@ -180,7 +187,8 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
       y = inner<T, DP>(vs + at, g, y);
 #pragma unroll
       for (int k = 0; k < 16; ++k)
-        y[k] *= exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[k >> 2][k & 3]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
+        y[k] *= exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[u][k]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
+      if (t + 1 < t1) fetch_bias(t + 1, u);
       if (word_u != 0xffffffffu) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) y[k] = (word_u >> (4 * h) >> acc_row(k, 0)) & 1 ? y[k] : 0.f;
@@ -219,6 +227,7 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
       sk.store(to, KS);
       sv.store(to + KT * KS, KS);
     }
+    now = next, next = then;
     __syncthreads();
   }
 
@@ -351,8 +360,25 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dk[0][dt] = zero16(), dv[0][dt] = zero16();
 
+  float bs[RT / 32][16];
+  auto fetch_bias = [&](int t, int u) __attribute__((always_inline)) {
+    if constexpr (BIAS) {
+      const int g = t / head_tiles, i0 = (t - g * head_tiles) * RT + 32 * u, head = hk * p.G + g;
+      const long ba = b * p.bb + head * p.bh + (i0 + 4 * h) * p.bq + key * p.bk;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        bs[u][k] = 0.f;
+        if (i0 + acc_row(k, h) < p.Lq && seen) {
+          const long e = ba + acc_row(k, 0) * p.bq;
+          bs[u][k] = p.bias_f32 ? ((const float*)p.bias)[e] : (float)((const T*)p.bias)[e];
+        }
+      }
+    }
+  };
   if (t0 < t1) {
     load_tile(t0);
+#pragma unroll
+    for (int u = 0; u < RT / 32; ++u) fetch_bias(t0, u);
     store_tile(t0);
   }
   __syncthreads();
@@ -365,19 +391,6 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
       for (int u = 0; u < RT / 32; ++u) {
         const int at = (32 * u + n) * S + M::E * h;
-        float bs[16];
-        if constexpr (BIAS) {
-          const int g = t / head_tiles, i0 = (t - g * head_tiles) * RT + 32 * u, head = hk * p.G + g;
-          const long ba = b * p.bb + head * p.bh + (i0 + 4 * h) * p.bq + key * p.bk;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            bs[k] = 0.f;
-            if (i0 + acc_row(k, h) < p.Lq && seen) {
-              const long e = ba + acc_row(k, 0) * p.bq;
-              bs[k] = p.bias_f32 ? ((const float*)p.bias)[e] : (float)((const T*)p.bias)[e];
-            }
-          }
-        }
         f32x16 pr = zero16(), dp;
         if constexpr (KLDS) {
 #pragma unroll
@@ -401,10 +414,11 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = 4 * run + e;
-            pr[k] = exp2_fast(BIAS ? fmaf(fmaf(pr[k], c, bs[k]) - m[e], LOG2E, P_UP - ll[e])
+            pr[k] = exp2_fast(BIAS ? fmaf(fmaf(pr[k], c, bs[u][k]) - m[e], LOG2E, P_UP - ll[e])
                                    : exponent<T>(pr[k], c, m[e]) + (P_UP - ll[e]));
           }
         }
+        if (t + 1 < t1) fetch_bias(t + 1, u);
         if (!all_seen) {
 #pragma unroll
           for (int k = 0; k < 16; ++k) pr[k] = seen ? pr[k] : 0.f;

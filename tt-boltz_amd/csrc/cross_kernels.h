@@ -213,16 +213,42 @@ struct Stage {
   }
 };
 
+// Which of a tile's KT keys are seen, a bit each, the same in every wave.  `fetch` asks for a tile's mask
+// bytes, `take` turns them into the bits an iteration later: nothing waits for them.
+template <int KT>
+struct Seen {
+  static constexpr int W = KT / 64;
+  uint64_t w[W];
+  uint8_t byte[W];
+  PF_DEV void fetch(int t, int len, const uint8_t* mask) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int key = t * KT + 64 * i + lane;
+      byte[i] = key < len ? (mask ? mask[key] : 1) : 0;
+    }
+  }
+  PF_DEV void take() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = __ballot(byte[i] != 0);
+  }
+  PF_DEV bool all() const {
+    uint64_t a = ~0ull;
+#pragma unroll
+    for (int i = 0; i < W; ++i) a &= w[i];
+    return a == ~0ull;
+  }
+  // bits of keys 32 k .. + 31
+  PF_DEV uint32_t part(int k) const { return (uint32_t)((W == 2 && k >= 2 ? w[W - 1] : w[0]) >> (32 * (k & 1))); }
+  PF_DEV bool at(int key) const { return ((W == 2 && key >= 64 ? w[W - 1] : w[0]) >> (key & 63)) & 1; }
+};
+
 // Key tile t of one key head: rows of hidden keys are zeros (what stands there, NaN say, takes no part).
 template <typename T, int DP, int KT>
-PF_DEV void load_keys(Stage<T, DP, KT>& s, const T* base, long stride, int D, int t, int len, const uint8_t* mask) {
+PF_DEV void load_keys(Stage<T, DP, KT>& s, const T* base, long stride, int D, int t, const Seen<KT>& seen) {
   const T* p = base + (long)t * KT * stride;
-  if (!mask && (t + 1) * KT <= len) s.load(p, stride, D);
-  else
-    s.load_some(p, stride, D, [&](int row) __attribute__((always_inline)) {
-      const int key = t * KT + row;
-      return key < len && (!mask || mask[key]);
-    });
+  if (seen.all()) s.load(p, stride, D);
+  else s.load_some(p, stride, D, [&](int row) __attribute__((always_inline)) { return seen.at(row); });
 }
 
 // Workgroup w runs on XCD w % 8: neighbouring ids go to one XCD, so the workgroups of a (batch, key head)
@@ -264,6 +290,17 @@ PF_DEV void load_bias(const XaParams& p, const char* row, int key, bool ok, floa
   if (!ok) return;
   if (p.bias_f32) load_bias4(reinterpret_cast<const float*>(row), key, p.Lk, p.bk == 1, p.bk, x);
   else load_bias4(reinterpret_cast<const T*>(row), key, p.Lk, p.bk == 1, p.bk, x);
+}
+// its keys key0 .. + 3, + 8 .. + 11, ..: a lane's 16 values of a 32-key tile
+template <typename T>
+PF_DEV void load_bias16(const XaParams& p, const char* row, int key0, bool ok, float (&x)[16]) {
+#pragma unroll
+  for (int run = 0; run < 4; ++run) {
+    float y[4];
+    load_bias<T>(p, row, key0 + 8 * run, ok, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * run + e] = y[e];
+  }
 }
 // a lane's row of the bias
 template <typename T>
@@ -309,7 +346,7 @@ template <typename T, int DP, bool BIAS, bool FEW, int R>
 constexpr int fwd_waves() {
   if (DP == 128) return FEW || __is_same(T, float) ? 1 : 2;
   if (R == 2) return 2;
-  return __is_same(T, float) ? 2 : DP == 64 ? (BIAS || FEW ? 3 : 4) : 4;
+  return __is_same(T, float) ? 2 : DP == 64 ? (BIAS ? 2 : FEW ? 3 : 4) : BIAS && !FEW ? 3 : 4;
 }
 
 template <typename T, int DP, bool BIAS, bool FEW, int R>
@@ -345,9 +382,10 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
   const T* const vb = (const T*)p.v + b * p.vb + hk * p.vh;
 
   Stage<T, DP, KT> sk, sv;
-  auto load_tile = [&](int t) __attribute__((always_inline)) {
-    load_keys(sk, kb, p.kl, p.D, t, len, mask);
-    load_keys(sv, vb, p.vl, p.D, t, len, mask);
+  Seen<KT> now, next;
+  auto load_tile = [&](int t, const Seen<KT>& seen) __attribute__((always_inline)) {
+    load_keys(sk, kb, p.kl, p.D, t, seen);
+    load_keys(sv, vb, p.vl, p.D, t, seen);
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;   // x in units of 1 (bias) or log2
@@ -362,8 +400,22 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
     for (int dt = 0; dt < DT; ++dt) o[r][dt] = zero16();
   }
 
+  // the next tile's bias is on its way while this one's softmax and product run
+  float bs[NSUB][R][16];
+  auto fetch_bias = [&](int t) __attribute__((always_inline)) {
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) load_bias16<T>(p, bias[r], t * KT + sub0 + 32 * u + 4 * h, row_ok[r], bs[u][r]);
+    }
+  };
   if (t0 < t1) {
-    load_tile(t0);
+    now.fetch(t0, len, mask);
+    next.fetch(t0 + 1, len, mask);
+    now.take();
+    load_tile(t0, now);
+    fetch_bias(t0);
     sk.store(ks0, KS);
     sv.store(ks0 + KT * KS, VS);
   }
@@ -371,31 +423,22 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
   for (int t = t0; t < t1; ++t) {
     const T* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
     const T* const vs = ks + KT * KS;
-    if (t + 1 < t1) load_tile(t + 1);
+    next.take();
+    if (t + 1 < t1) load_tile(t + 1, next);
+    Seen<KT> then;
+    then.fetch(t + 2, len, mask);
     // the keys of this wave that are seen, bit j: key sub0 + j of the tile
-    uint64_t word = ~0ull;
-    if (mask || (t + 1) * KT > len) {
-      const int key_l = t * KT + sub0 + (FEW ? n : lane);
-      word = __ballot(key_l < len && (!mask || mask[key_l]));
-    }
+    const uint64_t word = FEW ? now.part(wid) : now.w[0];
+    f32x16 x[NSUB][R];
     if (word) {
-      f32x16 x[NSUB][R];
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
-        float bs[R][4][4];
-        if constexpr (BIAS) {
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int run = 0; run < 4; ++run)
-              load_bias<T>(p, bias[r], t * KT + sub0 + 32 * u + 8 * run + 4 * h, row_ok[r], bs[r][run]);
-        }
         inner_rows<T, DP, R>(ks + (sub0 + 32 * u + n) * KS + M::E * h, q, x[u]);
         if constexpr (BIAS) {
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int k = 0; k < 16; ++k) x[u][r][k] = fmaf(x[u][r][k], c, bs[r][k >> 2][k & 3]);
+            for (int k = 0; k < 16; ++k) x[u][r][k] = fmaf(x[u][r][k], c, bs[u][r][k]);
         }
         const uint32_t w = (uint32_t)(word >> (FEW ? 0 : 32 * u));
         if (w != 0xffffffffu) {
@@ -405,6 +448,9 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
             for (int k = 0; k < 16; ++k) x[u][r][k] = (w >> (4 * h) >> acc_row(k, 0)) & 1 ? x[u][r][k] : -INFINITY;
         }
       }
+    }
+    if (t + 1 < t1) fetch_bias(t + 1);
+    if (word) {
       typename M::Packed pk[NSUB][R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -449,6 +495,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
       sk.store(to, KS);
       sv.store(to + KT * KS, VS);
     }
+    now = next, next = then;
     __syncthreads();
   }
 #pragma unroll
