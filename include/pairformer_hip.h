@@ -555,7 +555,7 @@ int pf_dropout_add_fwd(const pf_dropout_args* args);
  * against atoms; a decoder against an encoder):
  *   x_ij = scale q_i . k_j + bias_ij;  P = softmax over the keys that are seen;  o_i = sum_j P_ij v_j.
  * q [B][Lq][H][D] and k, v [B][Lk][Hk][D] in `dtype`, any strides that are multiples of 16 bytes with
- * contiguous channels; D a multiple of 8 up to 128; H / Hk heads share a key head.  Key j of batch
+ * contiguous channels (q_l, k_l, v_l and H D below 2^22); D a multiple of 8 up to 128; H / Hk heads share a key head.  Key j of batch
  * element b is seen where j < k_lens[b] (clamped to [0, Lk]) and mask[b][j] != 0 (either may be
  * NULL).  Hidden keys are not used, whatever stands there; a query that sees nothing (no key, or a
  * bias of -inf throughout) has o = 0 and no gradient.  bias: any strides, fp32 or dtype.

@@ -213,7 +213,7 @@ def test_cross_attention_abi_refuses_without_launching():
               v_b=224, v_l=32, v_h=16, o=d)
     for change, say in ((dict(dtype=5), "dtype"), (dict(D=20), "D must"), (dict(D=136), "D must"), (dict(H=3), "bad shape"),
                         (dict(Hk=0), "bad shape"), (dict(B=-1), "bad shape"), (dict(scale=float("nan")), "finite"), (dict(q=None), "null"),
-                        (dict(k=None), "null"), (dict(o=None), "null"), (dict(q=d + 4), "aligned"), (dict(k_l=34), "strides"),
+                        (dict(k=None), "null"), (dict(o=None), "null"), (dict(q=d + 4), "aligned"), (dict(k_l=34), "strides"), (dict(v_l=1 << 22), "below 2^22"),
                         (dict(o=d + 8), "aligned"), (dict(bias=d, bias_dtype=1), "bias"), (dict(Lk=1 << 30), "too long"),
                         (dict(B=1 << 20, Lq=1 << 20), "too large")):
         a = _lib.CrossAttnArgs(**{**ok, **change})

@@ -10,7 +10,8 @@ struct XaParams {
   int neg;
   float grad_scale;              // the caller's scale, a factor of dq and dk
   const void *q, *k, *v;
-  long qb, ql, qh, kb, kl, kh, vb, vl, vh;     // strides in elements, channels contiguous
+  long qb, qh, kb, kh, vb, vh;   // strides in elements, channels contiguous
+  int ql, kl, vl;                // (from row to row: below 2^22)
   const void* bias;
   int bias_f32;                  // fp32, else the element type
   long bb, bh, bq, bk;

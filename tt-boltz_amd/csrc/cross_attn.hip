@@ -43,6 +43,8 @@ int check_data(const pf_cross_attn_args* a, const char* fn) {
     return pf_fail(PF_E_INVALID, "%s: q, k and v must be 16-byte aligned", fn);
   for (long s : {a->q_b, a->q_l, a->q_h, a->k_b, a->k_l, a->k_h, a->v_b, a->v_l, a->v_h})
     if (s % unit) return pf_fail(PF_E_INVALID, "%s: strides must be multiples of 16 bytes", fn);
+  for (long s : {a->q_l, a->k_l, a->v_l, (long)a->H * a->D})
+    if (s < 0 || s >= 1l << 22) return pf_fail(PF_E_INVALID, "%s: row strides must be below 2^22 elements (got %ld)", fn, s);
   return PF_OK;
 }
 
@@ -54,14 +56,14 @@ XaParams params_of(const pf_cross_attn_args* a) {
   p.scale = __builtin_fabsf(a->scale);
   if (p.scale < 1e-30f) p.scale = 1e-30f;   // 0: all logits equal (0 times a hidden key's -inf would not be)
   p.q = a->q, p.k = a->k, p.v = a->v;
-  p.qb = a->q_b, p.ql = a->q_l, p.qh = a->q_h, p.kb = a->k_b, p.kl = a->k_l, p.kh = a->k_h;
-  p.vb = a->v_b, p.vl = a->v_l, p.vh = a->v_h;
+  p.qb = a->q_b, p.ql = (int)a->q_l, p.qh = a->q_h, p.kb = a->k_b, p.kl = (int)a->k_l, p.kh = a->k_h;
+  p.vb = a->v_b, p.vl = (int)a->v_l, p.vh = a->v_h;
   p.bias = a->bias, p.bias_f32 = a->bias_dtype == PF_FP32;
   p.bb = a->bias_b, p.bh = a->bias_h, p.bq = a->bias_q, p.bk = a->bias_k;
   p.mask = a->mask, p.mb = a->mask_b, p.lens = a->k_lens;
   p.o = a->o, p.o32 = a->o32;
   if (a->stats) p.st_m = a->stats, p.st_l = a->stats + (long)a->B * a->H * a->Lq;
-  p.few = p.rows <= 32;
+  p.few = p.rows <= 32 && !(a->dtype == PF_FP32 && p.D > 64);
   p.splits = p.per = 1;
   const int longest = p.rows > p.Lk ? p.rows : p.Lk;
   p.chunks = longest > 64 * 32 ? 64 : (longest + 31) / 32;

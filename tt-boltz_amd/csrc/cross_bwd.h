@@ -107,8 +107,9 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP);
   extern __shared__ __align__(16) char smem[];
-  constexpr int BUF = 2 * KT * KS, NBUF = buffers<T, FEW>();
-  T* const ks0 = reinterpret_cast<T*>(smem);
+  typedef typename M::L L;
+  constexpr int PK = KT * KS, BUF = 2 * M::PARTS * PK, NBUF = buffers<T, FEW>();
+  L* const ks0 = reinterpret_cast<L*>(smem);   // per buffer: the parts of the keys, then of the values
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
   constexpr int ROWS = FEW ? 32 : 128;
   const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
@@ -160,12 +161,12 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) fetch_bias(t0, u);
     sk.store(ks0, KS);
-    sv.store(ks0 + KT * KS, KS);
+    sv.store(ks0 + M::PARTS * PK, KS);
   }
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
-    const T* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
-    const T* const vs = ks + KT * KS;
+    const L* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    const L* const vs = ks + M::PARTS * PK;
     next.take();
     if (t + 1 < t1) load_tile(t + 1, next);
     Seen<KT> then;
@@ -180,11 +181,11 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
       }
       const int key0 = t * KT + sub0 + 32 * u + 4 * h;
       const int at = (sub0 + 32 * u + n) * KS + M::E * h;
-      const f32x16 s = inner<T, DP>(ks + at, q, zero16());
+      const f32x16 s = inner<T, DP>(ks + at, PK, q, zero16());
       f32x16 y;
 #pragma unroll
       for (int k = 0; k < 16; ++k) y[k] = -delta;
-      y = inner<T, DP>(vs + at, g, y);
+      y = inner<T, DP>(vs + at, PK, g, y);
 #pragma unroll
       for (int k = 0; k < 16; ++k)
         y[k] *= exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[u][k]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
@@ -218,14 +219,14 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
       }
       if (word_u) {
         const typename M::Packed pk[1] = {M::pack(y)};
-        M::template outer<DT, 1>(ks + (sub0 + 32 * u) * KS, KS, lane, pk, dq);
+        M::template outer<DT, 1>(ks + (sub0 + 32 * u) * KS, PK, KS, lane, pk, dq);
       }
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) {
-      T* const to = ks0 + (NBUF == 2 ? (t + 1 - t0) % 2 * BUF : 0);
+      L* const to = ks0 + (NBUF == 2 ? (t + 1 - t0) % 2 * BUF : 0);
       sk.store(to, KS);
-      sv.store(to + KT * KS, KS);
+      sv.store(to + M::PARTS * PK, KS);
     }
     now = next, next = then;
     __syncthreads();
@@ -292,19 +293,22 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
 // ------------------------------------------------------------------------------ dk, dv
 // 4 waves x 32 keys; a tile is RT consecutive queries of one head, the heads of the key head one after
 // the other.  A wave's values stay in registers; its keys do too where those suffice for two waves per
-// SIMD, else (128 channels) they are read from LDS for each tile.
+// SIMD, else (128 channels, fp32 from 64) they are read from LDS for each tile
+// (fp32: without padding, so that two workgroups share a CU's LDS; the 16-byte pieces of a row are
+// permuted by the row's low bits instead, and 16 rows still land on distinct banks).
 template <typename T, int DP>
-constexpr bool keys_in_lds() { return DP == 128 && !__is_same(T, float); }
+constexpr bool keys_in_lds() { return DP == 128 || (Mma<T>::SPLIT && DP == 64); }
 
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void xa_dkv_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::row_stride(DP);
-  constexpr int NBUF = buffers<T, false>(), STATS = 3 * RT * 4 / (int)sizeof(T), BUF = 2 * RT * S + STATS;
+  typedef typename M::L L;
+  constexpr int PT = RT * S, STATS = 3 * RT * 2, NBUF = buffers<T, false>(), BUF = 2 * M::PARTS * PT + STATS;
   constexpr bool KLDS = keys_in_lds<T, DP>();
   extern __shared__ __align__(16) char smem[];
-  T* const buf0 = reinterpret_cast<T*>(smem);   // per buffer: q, do, then fp32 [3][RT] maximum, log2 of the sum, delta
-  T* const kl = buf0 + NBUF * BUF;
+  L* const buf0 = reinterpret_cast<L*>(smem);   // per buffer: q, do, then fp32 [3][RT] maximum, log2 of the sum, delta
+  L* const kl = buf0 + NBUF * BUF;              // parts of the keys
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
   const Block blk = block_of(p, (p.Lk + XA_KEYS - 1) / XA_KEYS);
   const int b = blk.b, hk = blk.hk;
@@ -315,10 +319,16 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
   Frag<T, DP> kf, vf;
   kf.load((const T*)p.k + b * p.kb + (long)key * p.kl + hk * p.kh, p.D, h, seen, p.neg);
   vf.load((const T*)p.v + b * p.vb + (long)key * p.vl + hk * p.vh, p.D, h, seen);
-  T* const kl_row = kl + (32 * wid + n) * S + M::E * h;
+  constexpr int KLS = M::SPLIT ? DP : S;
+  auto kl_at = [&](int s) __attribute__((always_inline)) {
+    const int piece = M::SPLIT ? (2 * s + h) ^ (n & (DP / 8 - 1)) : 2 * s + h;
+    return kl + (32 * wid + n) * KLS + 8 * piece;
+  };
   if constexpr (KLDS) {
 #pragma unroll
-    for (int s = 0; s < Frag<T, DP>::S; ++s) *reinterpret_cast<typename M::frag_t*>(kl_row + M::CH * s) = kf.f[s];
+    for (int s = 0; s < Frag<T, DP>::S; ++s)
+#pragma unroll
+      for (int k = 0; k < M::PARTS; ++k) *reinterpret_cast<typename M::part_t*>(kl_at(s) + k * XA_KEYS * KLS) = kf.f[s].p[k];
   }
   const float sf = SCALED<T> ? ds_scale(p, b, hk) : 1.f;
   constexpr float P_UP = SCALED<T> ? 15.f : 0.f, P_FACTOR = SCALED<T> ? 32768.f : 1.f;
@@ -337,11 +347,11 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
     const T* gp = (const T*)p.dout + (((long)b * p.Lq + i0) * p.H + head) * p.D;
     if (left >= RT) {
       sq.load(qp, p.ql, p.D);
-      sg.load(gp, (long)p.H * p.D, p.D);
+      sg.load(gp, p.H * p.D, p.D);
     } else {
       auto there = [&](int row) __attribute__((always_inline)) { return row < left; };
       sq.load_some(qp, p.ql, p.D, there);
-      sg.load_some(gp, (long)p.H * p.D, p.D, there);
+      sg.load_some(gp, p.H * p.D, p.D, there);
     }
     if (sw < 3) {
       stat = sw == 1 ? INFINITY : 0.f;   // a row behind the last: P = 0
@@ -349,10 +359,10 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
     }
   };
   auto store_tile = [&](int t) __attribute__((always_inline)) {
-    T* const to = buf0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    L* const to = buf0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
     sq.store(to, S);
-    sg.store(to + RT * S, S);
-    if (sw < 3) reinterpret_cast<float*>(to + 2 * RT * S)[sw * RT + sr] = stat;
+    sg.store(to + M::PARTS * PT, S);
+    if (sw < 3) reinterpret_cast<float*>(to + 2 * M::PARTS * PT)[sw * RT + sr] = stat;
   };
 
   const float c = BIAS ? p.scale : p.scale * LOG2E;
@@ -383,9 +393,9 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
   }
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
-    const T* const qs = buf0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
-    const T* const gs = qs + RT * S;
-    const float* const st = reinterpret_cast<const float*>(gs + RT * S);
+    const L* const qs = buf0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    const L* const gs = qs + M::PARTS * PT;
+    const float* const st = reinterpret_cast<const float*>(gs + M::PARTS * PT);
     if (t + 1 < t1) load_tile(t + 1);
     if (any_seen) {
 #pragma unroll
@@ -395,10 +405,9 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
         if constexpr (KLDS) {
 #pragma unroll
           for (int s = 0; s < Frag<T, DP>::S; ++s)
-            pr = M::mma(*reinterpret_cast<const typename M::frag_t*>(qs + at + M::CH * s),
-                        *reinterpret_cast<const typename M::frag_t*>(kl_row + M::CH * s), pr);
+            pr = M::mma(M::load(qs + at + 16 * s, PT), M::load(kl_at(s), XA_KEYS * KLS), pr);
         } else {
-          pr = inner<T, DP>(qs + at, kf, pr);
+          pr = inner<T, DP>(qs + at, PT, kf, pr);
         }
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
@@ -406,7 +415,7 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
           for (int e = 0; e < 4; ++e) dp[4 * run + e] = -dl[e];
         }
-        dp = inner<T, DP>(gs + at, vf, dp);
+        dp = inner<T, DP>(gs + at, PT, vf, dp);
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
           const f32x4 m = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * run + 4 * h);
@@ -426,8 +435,8 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
         for (int k = 0; k < 16; ++k) dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
         const typename M::Packed pv[1] = {M::pack(pr)}, pd[1] = {M::pack(dp)};
-        M::template outer<DT, 1>(gs + 32 * u * S, S, lane, pv, dv);
-        M::template outer<DT, 1>(qs + 32 * u * S, S, lane, pd, dk);
+        M::template outer<DT, 1>(gs + 32 * u * S, PT, S, lane, pv, dv);
+        M::template outer<DT, 1>(qs + 32 * u * S, PT, S, lane, pd, dk);
       }
     }
     if constexpr (NBUF == 1) __syncthreads();
@@ -496,7 +505,7 @@ int sum_launch(const float* part, long step, int splits, void* out0, void* out1,
 template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
 int dq_launch(const XaParams& p, hipStream_t st) {
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
-  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * sizeof(T) * buffers<T, FEW>(), join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0;
+  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * 2 * Mma<T>::PARTS * buffers<T, FEW>(), join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0;
   const size_t lds = tiles > join ? tiles : join;
   if (int rc = pf_reserve_lds((const void*)xa_dq_kernel<T, DP, BIAS, FEW, DELTA>, lds, "xa_dq_kernel")) return rc;
   const int rt = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
@@ -508,33 +517,36 @@ int dq_launch(const XaParams& p, hipStream_t st) {
                : sum_launch<T>(p.part, rows * p.D, p.splits, p.dq, nullptr, rows * p.D, st);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool DELTA>
 int dq_dp(const XaParams& p, hipStream_t st) {
-  if (p.bias) return p.few ? dq_launch<T, DP, true, true, false>(p, st) : dq_launch<T, DP, true, false, false>(p, st);
-  return p.few ? dq_launch<T, DP, false, true, false>(p, st) : dq_launch<T, DP, false, false, false>(p, st);
+  if constexpr (has_few<T, DP>()) {
+    if (p.few && p.bias) return dq_launch<T, DP, true, true, DELTA>(p, st);
+    if constexpr (!DELTA) {
+      if (p.few) return dq_launch<T, DP, false, true, false>(p, st);
+    }
+  }
+  if constexpr (!DELTA) {
+    if (!p.bias) return dq_launch<T, DP, false, false, false>(p, st);
+  }
+  return dq_launch<T, DP, true, false, DELTA>(p, st);
 }
 
 // delta of 16-bit types with a bias gradient (part: where the splits go, delta itself if there is one)
-template <typename T, int DP>
-int exact_delta_dp(const XaParams& p, hipStream_t st) {
-  return p.few ? dq_launch<T, DP, true, true, true>(p, st) : dq_launch<T, DP, true, false, true>(p, st);
-}
-
 template <typename T>
 int exact_delta_type(const XaParams& p, hipStream_t st) {
-  return p.D <= 32 ? exact_delta_dp<T, 32>(p, st) : p.D <= 64 ? exact_delta_dp<T, 64>(p, st) : exact_delta_dp<T, 128>(p, st);
+  return p.D <= 32 ? dq_dp<T, 32, true>(p, st) : p.D <= 64 ? dq_dp<T, 64, true>(p, st) : dq_dp<T, 128, true>(p, st);
 }
 
 template <typename T>
 int dq_type(const XaParams& p, hipStream_t st) {
-  return p.D <= 32 ? dq_dp<T, 32>(p, st) : p.D <= 64 ? dq_dp<T, 64>(p, st) : dq_dp<T, 128>(p, st);
+  return p.D <= 32 ? dq_dp<T, 32, false>(p, st) : p.D <= 64 ? dq_dp<T, 64, false>(p, st) : dq_dp<T, 128, false>(p, st);
 }
 
 template <typename T, int DP, bool BIAS>
 int dkv_launch(const XaParams& p, hipStream_t st) {
   constexpr int RT = xa_rt(DP, __is_same(T, float)), S = Mma<T>::row_stride(DP);
-  const size_t lds = buffers<T, false>() * ((size_t)2 * RT * S * sizeof(T) + 3 * RT * 4) +
-                     (keys_in_lds<T, DP>() ? (size_t)XA_KEYS * S * sizeof(T) : 0);
+  const size_t lds = buffers<T, false>() * ((size_t)4 * Mma<T>::PARTS * RT * S + 3 * RT * 4) +
+                     (keys_in_lds<T, DP>() ? (size_t)2 * Mma<T>::PARTS * XA_KEYS * (Mma<T>::SPLIT ? DP : S) : 0);
   if (int rc = pf_reserve_lds((const void*)xa_dkv_kernel<T, DP, BIAS>, lds, "xa_dkv_kernel")) return rc;
   const int tiles = (p.Lk + XA_KEYS - 1) / XA_KEYS;
   xa_dkv_kernel<T, DP, BIAS><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);

@@ -4,7 +4,7 @@
 //   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (do_i . v_j - delta_i),  delta_i = do_i . o_i,
 //   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dbias = dS
 //
-// Every product runs on 32x32 MFMA tiles (accumulators: lane l, register r hold column l & 31, row
+// Every product runs on 32x32x16 MFMA tiles (accumulators: lane l, register r hold column l & 31, row
 // 8 (r >> 2) + 4 (l >> 5) + (r & 3)).  The forward and the dq kernel form S^T = K Q^T, so a lane's
 // column is one query: its softmax statistics are the lane's own, and the accumulator of P^T (dS^T)
 // is, as it stands, the right operand of O^T = V^T P^T (dQ^T = K^T dS^T), with the left operand read
@@ -33,133 +33,185 @@ PF_DEV float xor32_sum(float v) { return v + __shfl_xor(v, 32); }
 PF_DEV int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
 // ------------------------------------------------------------------------------ tiles
-// Frag<DP>: 32 rows x DP channels as an MFMA operand of products over channels.  Lane (n, h) holds of
-// row n, per step s, the 16 bytes at channel CH s + h * CH / 2 (CH channels a step: 16 of 16 bits,
-// 8 fp32; the two halves of the wave hold the step's two halves).
+// Operands of 16-bit types are themselves.  fp32 operands are split into three bf16 parts, each the
+// rounded rest of the ones before: x = h + m + l exactly, in bf16's exponent range, which is fp32's.  A
+// product takes h h', h m', m h', m m', h l' and l h'; what is left out is below 2^-25 of it.  Six bf16
+// MFMAs (192 cycles for 16 channels) take the place of eight fp32 ones (512).
+//
+// Op: 32 rows x 16 channels as an MFMA operand; lane (n, h) holds channels 8 h .. 8 h + 7 of row n.
+template <typename T>
+struct LdsType { typedef T type; };
+template <>
+struct LdsType<float> { typedef bhalf_t type; };
+
 template <typename T>
 struct Mma {
-  typedef T frag_t __attribute__((ext_vector_type(8)));
-  typedef T quad_t __attribute__((ext_vector_type(4)));
-  static constexpr int CH = 16, E = 8;
+  static constexpr bool SPLIT = __is_same(T, float);
+  static constexpr int PARTS = SPLIT ? 3 : 1, E = 8;
+  typedef typename LdsType<T>::type L;   // what LDS tiles hold, PARTS planes of it
+  typedef L part_t __attribute__((ext_vector_type(8)));
+  typedef L quad_t __attribute__((ext_vector_type(4)));
+  struct Op { part_t p[PARTS]; };
+  struct Packed { Op f[2]; };   // an accumulator as the right operand of a product over its 32 rows
+
   static constexpr int row_stride(int dp) { return dp + 8; }   // rows land on distinct banks (16 lanes x 16 bytes)
-  // only read in transposed 4 x 16 blocks: four rows x 32 channels on distinct banks
-  static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp == 64 ? 80 : dp + 32; }
-  static PF_DEV f32x16 mma(const frag_t& a, const frag_t& b, const f32x16& c) {
-    if constexpr (__is_same(T, half_t)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  // only read in transposed 4 x 16 blocks: four rows x 32 channels on (nearly) distinct banks
+  static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp == 64 ? 80 : dp + (SPLIT ? 8 : 32); }
+
+  static PF_DEV f32x16 mma1(const part_t& a, const part_t& b, const f32x16& c) {
+    if constexpr (__is_same(L, half_t)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // an accumulator as the right operand of a product over its 32 rows
-  struct Packed { frag_t f[2]; };
-  static PF_DEV Packed pack(const f32x16& p) {
+  static PF_DEV f32x16 mma(const Op& a, const Op& b, f32x16 c) {
+    if constexpr (SPLIT) {
+      c = mma1(a.p[2], b.p[0], c);
+      c = mma1(a.p[0], b.p[2], c);
+      c = mma1(a.p[1], b.p[1], c);
+      c = mma1(a.p[1], b.p[0], c);
+      c = mma1(a.p[0], b.p[1], c);
+    }
+    return mma1(a.p[0], b.p[0], c);
+  }
+  // x[i] into element i of p[0 .. PARTS)
+  template <int N, typename V>
+  static PF_DEV void put(const float (&x)[N], V* p) {
+    if constexpr (!SPLIT) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) p[0][i] = (L)x[i];
+    } else {
+      float r[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        p[0][i] = (L)x[i];
+        r[i] = x[i] - (float)p[0][i];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        p[1][i] = (L)r[i];
+        p[2][i] = (L)(r[i] - (float)p[1][i]);
+      }
+    }
+  }
+  // the same for a caller's values: infinities, and what rounds to one, are not split
+  template <int N, typename V>
+  static PF_DEV void put_any(const float (&x)[N], V* p) {
+    put(x, p);
+    if constexpr (SPLIT) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) top = fmaxf(top, __builtin_fabsf(x[i]));
+      if (top >= 3.38e38f) {   // bf16's largest value is 3.3895e38
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (__builtin_fabsf(x[i]) >= 3.38e38f) {
+            const float t = __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u), r = x[i] == t ? 0.f : x[i] - t;
+            p[0][i] = (L)t, p[1][i] = (L)r, p[2][i] = (L)(r - (float)p[1][i]);
+          }
+        }
+      }
+    }
+  }
+  static PF_DEV Packed pack(const f32x16& x) {
     Packed b;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 2; ++s) {
+      float y[8];
 #pragma unroll
-      for (int t = 0; t < 8; ++t) b.f[s][t] = (T)p[8 * s + t];
+      for (int t = 0; t < 8; ++t) y[t] = x[8 * s + t];
+      put(y, b.f[s].p);
+    }
     return b;
   }
-  // c + the sum of this lane's 16 values as they were rounded
+  // 16-bit types: c + the sum of this lane's 16 values as they were rounded
   static PF_DEV float sum(const Packed& b, float c) {
-    typedef T pair_t __attribute__((ext_vector_type(2)));
-    const pair_t one = {(T)1.f, (T)1.f};
+    typedef L pair_t __attribute__((ext_vector_type(2)));
+    const pair_t one = {(L)1.f, (L)1.f};
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int t = 0; t < 8; t += 2) {
-        const pair_t v = {b.f[s][t], b.f[s][t + 1]};
-        if constexpr (__is_same(T, half_t)) c = __builtin_amdgcn_fdot2(v, one, c, false);
+        const pair_t v = {b.f[s].p[0][t], b.f[s].p[0][t + 1]};
+        if constexpr (__is_same(L, half_t)) c = __builtin_amdgcn_fdot2(v, one, c, false);
         else c = __builtin_amdgcn_fdot2_f32_bf16(v, one, c, false);
       }
     return c;
   }
+  // LDS tiles are PARTS planes, `plane` elements apart
+  static PF_DEV Op load(const L* a, int plane) {
+    Op o;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) o.p[i] = *reinterpret_cast<const part_t*>(a + i * plane);
+    return o;
+  }
   // acc[r][dt] += X^T P[r] over 32 rows of the LDS tile X (row stride `st`), taken in P's order.  A transposing
   // read hands lane i of 16 the column i of a 4 x 16 block whose 8-byte pieces the lanes point at.
   template <int DT, int R>
-  static PF_DEV void outer(const T* x, int st, int lane, const Packed (&p)[R], f32x16 (&acc)[R][DT]) {
+  static PF_DEV void outer(const L* x, int plane, int st, int lane, const Packed (&p)[R], f32x16 (&acc)[R][DT]) {
     const int h = lane >> 5, i = lane & 15, c16 = (lane >> 4) & 1;
-    const T* at = x + (4 * h + (i >> 2)) * st + 16 * c16 + 4 * (i & 3);
+    const L* at = x + (4 * h + (i >> 2)) * st + 16 * c16 + 4 * (i & 3);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const quad_t lo = tr_read(at + (16 * s) * st + 32 * dt), hi = tr_read(at + (16 * s + 8) * st + 32 * dt);
-        const frag_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        Op a;
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+          const L* pl = at + k * plane + 32 * dt;
+          const quad_t lo = tr_read(pl + (16 * s) * st), hi = tr_read(pl + (16 * s + 8) * st);
+          a.p[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][dt] = mma(a, p[r].f[s], acc[r][dt]);
       }
   }
-  static PF_DEV quad_t tr_read(const T* p) {
+  static PF_DEV quad_t tr_read(const L* p) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_t;
     return __builtin_bit_cast(quad_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p));
   }
 };
 
-template <>
-struct Mma<float> {
-  typedef f32x4 frag_t;
-  static constexpr int CH = 8, E = 4;
-  static constexpr int row_stride(int dp) { return dp + 4; }
-  static constexpr int col_stride(int dp) { return dp + 4; }
-  static PF_DEV f32x16 mma(const frag_t& a, const frag_t& b, f32x16 c) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-    return c;
-  }
-  typedef f32x16 Packed;
-  static PF_DEV Packed pack(const f32x16& p) { return p; }
-  static PF_DEV float sum(const Packed& b, float c) {
-#pragma unroll
-    for (int t = 0; t < 16; ++t) c += b[t];
-    return c;
-  }
-  template <int DT, int R>
-  static PF_DEV void outer(const float* x, int st, int lane, const f32x16 (&p)[R], f32x16 (&acc)[R][DT]) {
-    const int h = lane >> 5, n = lane & 31;
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const float a = x[acc_row(k, h) * st + 32 * dt + n];
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[r][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r][k], acc[r][dt], 0, 0, 0);
-      }
-  }
-};
-
+// 32 rows x DP channels in registers
 template <typename T, int DP>
 struct Frag {
-  static constexpr int S = DP / Mma<T>::CH;
-  typename Mma<T>::frag_t f[S];
+  static constexpr int S = DP / 16;
+  typename Mma<T>::Op f[S];
   // row `p` in global memory; channels >= D are zero, and all are where !ok
   PF_DEV void load(const T* p, int D, int h, bool ok, bool neg = false) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int d = Mma<T>::CH * s + Mma<T>::E * h;
-      typename Mma<T>::frag_t z = {};
-      f[s] = ok && d < D ? *reinterpret_cast<const typename Mma<T>::frag_t*>(p + d) : z;
-      if (neg) f[s] = -f[s];
+      const int d = 16 * s + 8 * h;
+      if constexpr (Mma<T>::SPLIT) {
+        f32x4 a = {}, b = {};
+        if (ok && d < D) a = *reinterpret_cast<const f32x4*>(p + d), b = *reinterpret_cast<const f32x4*>(p + d + 4);
+        const float g = neg ? -1.f : 1.f;
+        const float x[8] = {a[0] * g, a[1] * g, a[2] * g, a[3] * g, b[0] * g, b[1] * g, b[2] * g, b[3] * g};
+        Mma<T>::put_any(x, f[s].p);
+      } else {
+        const typename Mma<T>::part_t z = {};
+        f[s].p[0] = ok && d < D ? *reinterpret_cast<const typename Mma<T>::part_t*>(p + d) : z;
+        if (neg) f[s].p[0] = -f[s].p[0];
+      }
     }
   }
 };
 
-// c += A B^T over channels: A the LDS tile's 32 rows at `a` (this lane's row, channel E h), B a fragment
+// c += A B^T over channels: A the LDS tile's 32 rows at `a` (this lane's row, channel 8 h), B a fragment
 template <typename T, int DP>
-PF_DEV f32x16 inner(const T* a, const Frag<T, DP>& b, f32x16 c) {
+PF_DEV f32x16 inner(const typename Mma<T>::L* a, int plane, const Frag<T, DP>& b, f32x16 c) {
 #pragma unroll
-  for (int s = 0; s < Frag<T, DP>::S; ++s)
-    c = Mma<T>::mma(*reinterpret_cast<const typename Mma<T>::frag_t*>(a + Mma<T>::CH * s), b.f[s], c);
+  for (int s = 0; s < Frag<T, DP>::S; ++s) c = Mma<T>::mma(Mma<T>::load(a + 16 * s, plane), b.f[s], c);
   return c;
 }
 
-// c[r] = A B[r]^T over channels: A the LDS tile's 32 rows at `a` (this lane's row, channel E h)
+// c[r] = A B[r]^T
 template <typename T, int DP, int R>
-PF_DEV void inner_rows(const T* a, const Frag<T, DP> (&b)[R], f32x16 (&c)[R]) {
+PF_DEV void inner_rows(const typename Mma<T>::L* a, int plane, const Frag<T, DP> (&b)[R], f32x16 (&c)[R]) {
 #pragma unroll
   for (int r = 0; r < R; ++r) c[r] = zero16();
 #pragma unroll
   for (int s = 0; s < Frag<T, DP>::S; ++s) {
-    const auto f = *reinterpret_cast<const typename Mma<T>::frag_t*>(a + Mma<T>::CH * s);
+    const auto f = Mma<T>::load(a + 16 * s, plane);
 #pragma unroll
     for (int r = 0; r < R; ++r) c[r] = Mma<T>::mma(f, b[r].f[s], c[r]);
   }
@@ -170,46 +222,51 @@ PF_DEV void inner_rows(const T* a, const Frag<T, DP> (&b)[R], f32x16 (&c)[R]) {
 template <typename T, int DP, int ROWS>
 struct Stage {
   typedef typename Vec16<T>::type vec_t;
+  typedef typename Mma<T>::L L;
   static constexpr int N = Vec16<T>::N, PER = DP / N, CH = ROWS * PER / 256, STEP = 256 / PER;
   static_assert(ROWS * PER % 256 == 0 && 256 % PER == 0, "whole pieces per thread");
   vec_t v[CH];
   static PF_DEV int row(int j) { return (int)threadIdx.x / PER + j * STEP; }
   static PF_DEV int chan() { return (int)threadIdx.x % PER * N; }
+  // this thread's first piece, in bytes from the tile's first row (row strides are below 2^22 elements)
+  static PF_DEV uint32_t first(int stride) { return (uint32_t)((row(0) * stride + chan()) * (int)sizeof(T)); }
   // p: row 0 of the tile, rows `stride` apart; all rows are there
-  PF_DEV void load(const T* p, long stride, int D) {
-    const vec_t z = {};
+  PF_DEV void load(const T* p, int stride, int D) {
     if (chan() < D) {
-      p += row(0) * stride + chan();
+      const uint32_t at = first(stride);
 #pragma unroll
-      for (int j = 0; j < CH; ++j) v[j] = *reinterpret_cast<const vec_t*>(p + j * STEP * stride);
+      for (int j = 0; j < CH; ++j) v[j] = *reinterpret_cast<const vec_t*>(reinterpret_cast<const char*>(p + j * STEP * stride) + at);
     } else {
+      const vec_t z = {};
 #pragma unroll
       for (int j = 0; j < CH; ++j) v[j] = z;
     }
   }
-  // rows with bit row(j) of `rows(j)` only, zeros for the others
+  // the rows for which there(row) holds, zeros for the others
   template <typename F>
-  PF_DEV void load_some(const T* p, long stride, int D, F there) {
-    p += row(0) * stride + chan();
+  PF_DEV void load_some(const T* p, int stride, int D, F there) {
+    const uint32_t at = first(stride);
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const vec_t z = {};
-      v[j] = chan() < D && there(row(j)) ? *reinterpret_cast<const vec_t*>(p + j * STEP * stride) : z;
+      v[j] = chan() < D && there(row(j))
+                 ? *reinterpret_cast<const vec_t*>(reinterpret_cast<const char*>(p + j * STEP * stride) + at) : z;
     }
   }
-  // row(r): its address, or null (zeros)
-  template <typename F>
-  PF_DEV void gather(int D, F at) {
+  PF_DEV void store(L* lds, int stride) const {
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      const T* p = at(row(j));
-      const vec_t z = {};
-      v[j] = p && chan() < D ? *reinterpret_cast<const vec_t*>(p + chan()) : z;
-    }
-  }
-  PF_DEV void store(T* lds, int stride) const {
+      L* const to = lds + row(j) * stride + chan();
+      if constexpr (Mma<T>::SPLIT) {
+        typename Mma<T>::quad_t q[3];
+        const float x[4] = {v[j][0], v[j][1], v[j][2], v[j][3]};
+        Mma<T>::put_any(x, q);
 #pragma unroll
-    for (int j = 0; j < CH; ++j) *reinterpret_cast<vec_t*>(lds + row(j) * stride + chan()) = v[j];
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<typename Mma<T>::quad_t*>(to + k * ROWS * stride) = q[k];
+      } else {
+        *reinterpret_cast<vec_t*>(to) = v[j];
+      }
+    }
   }
 };
 
@@ -245,7 +302,7 @@ struct Seen {
 
 // Key tile t of one key head: rows of hidden keys are zeros (what stands there, NaN say, takes no part).
 template <typename T, int DP, int KT>
-PF_DEV void load_keys(Stage<T, DP, KT>& s, const T* base, long stride, int D, int t, const Seen<KT>& seen) {
+PF_DEV void load_keys(Stage<T, DP, KT>& s, const T* base, int stride, int D, int t, const Seen<KT>& seen) {
   const T* p = base + (long)t * KT * stride;
   if (seen.all()) s.load(p, stride, D);
   else s.load_some(p, stride, D, [&](int row) __attribute__((always_inline)) { return seen.at(row); });
@@ -355,8 +412,9 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP), VS = M::col_stride(DP);
   extern __shared__ __align__(16) char smem[];
-  constexpr int BUF = KT * (KS + VS), NBUF = buffers<T, FEW>();
-  T* const ks0 = reinterpret_cast<T*>(smem);
+  typedef typename M::L L;
+  constexpr int PK = KT * KS, PV = KT * VS, BUF = M::PARTS * (PK + PV), NBUF = buffers<T, FEW>();
+  L* const ks0 = reinterpret_cast<L*>(smem);   // per buffer: the parts of the keys, then of the values
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
   constexpr int ROWS = FEW ? 32 : 128 * R;
   const Block blk = block_of(p, (p.rows + ROWS - 1) / ROWS);
@@ -417,12 +475,12 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
     load_tile(t0, now);
     fetch_bias(t0);
     sk.store(ks0, KS);
-    sv.store(ks0 + KT * KS, VS);
+    sv.store(ks0 + M::PARTS * PK, VS);
   }
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
-    const T* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
-    const T* const vs = ks + KT * KS;
+    const L* const ks = ks0 + (NBUF == 2 ? (t - t0) % 2 * BUF : 0);
+    const L* const vs = ks + M::PARTS * PK;
     next.take();
     if (t + 1 < t1) load_tile(t + 1, next);
     Seen<KT> then;
@@ -433,7 +491,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
     if (word) {
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
-        inner_rows<T, DP, R>(ks + (sub0 + 32 * u + n) * KS + M::E * h, q, x[u]);
+        inner_rows<T, DP, R>(ks + (sub0 + 32 * u + n) * KS + M::E * h, PK, q, x[u]);
         if constexpr (BIAS) {
 #pragma unroll
           for (int r = 0; r < R; ++r)
@@ -478,7 +536,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
 #pragma unroll
           for (int k = 0; k < 16; ++k) pr[k] = exp2_fast(BIAS ? (x[u][r][k] - mu) * LOG2E : exponent<T>(x[u][r][k], c, mu));
           pk[u][r] = M::pack(pr);
-          if constexpr (BIAS) {   // the bias's gradient wants P, and so the sum, to fp32
+          if constexpr (BIAS || M::SPLIT) {   // a bias's gradient wants P, and so the sum, to fp32
 #pragma unroll
             for (int k = 0; k < 16; ++k) l[r] += pr[k];
           } else {
@@ -487,13 +545,13 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
         }
       }
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u) M::template outer<DT, R>(vs + (sub0 + 32 * u) * VS, VS, lane, pk[u], o);
+      for (int u = 0; u < NSUB; ++u) M::template outer<DT, R>(vs + (sub0 + 32 * u) * VS, PV, VS, lane, pk[u], o);
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) {
-      T* const to = ks0 + (NBUF == 2 ? (t + 1 - t0) % 2 * BUF : 0);
+      L* const to = ks0 + (NBUF == 2 ? (t + 1 - t0) % 2 * BUF : 0);
       sk.store(to, KS);
-      sv.store(to + KT * KS, VS);
+      sv.store(to + M::PARTS * PK, VS);
     }
     now = next, next = then;
     __syncthreads();
@@ -637,7 +695,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(XaParams p) {
 template <typename T, int DP, bool FEW>
 size_t fwd_lds() {
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
-  const size_t tiles = (size_t)KT * (Mma<T>::row_stride(DP) + Mma<T>::col_stride(DP)) * sizeof(T) * buffers<T, FEW>();
+  const size_t tiles = (size_t)KT * (Mma<T>::row_stride(DP) + Mma<T>::col_stride(DP)) * 2 * Mma<T>::PARTS * buffers<T, FEW>();
   const size_t join = FEW ? (size_t)4 * 32 * (DP + 4 + 2) * 4 : 0;
   return tiles > join ? tiles : join;
 }
@@ -658,11 +716,17 @@ int fwd_launch(const XaParams& p, hipStream_t st) {
   return PF_OK;
 }
 
+// Whether the waves of a workgroup may share a row tile: three parts of 128 keys x 128 channels exceed LDS.
+template <typename T, int DP>
+constexpr bool has_few() { return !(Mma<T>::SPLIT && DP == 128); }
+
 template <typename T, int DP>
 int fwd_dp(const XaParams& p, hipStream_t st) {
-  if (p.bias) return p.few ? fwd_launch<T, DP, true, true, 1>(p, st) : fwd_launch<T, DP, true, false, 1>(p, st);
-  if (p.few) return fwd_launch<T, DP, false, true, 1>(p, st);
-  if constexpr (DP == 64 && sizeof(T) == 2) {
+  if constexpr (has_few<T, DP>()) {
+    if (p.few) return p.bias ? fwd_launch<T, DP, true, true, 1>(p, st) : fwd_launch<T, DP, false, true, 1>(p, st);
+  }
+  if (p.bias) return fwd_launch<T, DP, true, false, 1>(p, st);
+  if constexpr (DP == 64 && !Mma<T>::SPLIT) {
     if (p.wide) return fwd_launch<T, DP, false, false, 2>(p, st);
   }
   return fwd_launch<T, DP, false, false, 1>(p, st);

@@ -79,9 +79,9 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
     """``t`` [., ., ., D] where the kernels can read it in 16-byte pieces of its last dimension, else a copy."""
     s0, s1, s2, s3 = t.stride()
     unit = 3 if t.dtype == torch.float32 else 7
-    if s3 == 1 and not (s0 | s1 | s2) & unit and not t.data_ptr() & 15 and not t.is_neg():
+    if s3 == 1 and not (s0 | s1 | s2) & unit and not t.data_ptr() & 15 and s1 < 1 << 22 and not t.is_neg():
         return t
-    if (t.is_neg() or t.data_ptr() & 15 or s3 != 1
+    if (t.is_neg() or t.data_ptr() & 15 or s3 != 1 or (s1 >= 1 << 22 and t.shape[1] > 1)
             or any(s & unit for n, s in zip(t.shape, (s0, s1, s2)) if n > 1)):
         return t.resolve_neg().clone(memory_format=torch.contiguous_format)
     return t
