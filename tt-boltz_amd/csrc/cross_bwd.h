@@ -124,6 +124,7 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
   g.load((const T*)p.dout + row_at * p.D, p.D, h, row_ok);
   const long stat = ((long)b * p.H + head) * p.Lq + i;
   const float m = row_ok ? p.st_m[stat] : 0.f, ll = row_ok ? p.st_l[stat] : INFINITY;
+  const float m_ll = m + ll;   // 16-bit types without a bias (2^-24 of the logit is nothing there)
   const float delta = !DELTA && row_ok ? p.delta[stat] : 0.f;
   const float sf = SCALED<T> && !DELTA ? ds_scale(p, b, hk) : 1.f;
   float sum = 0.f;   // DELTA: this lane's half of the keys
@@ -188,7 +189,8 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
       y = inner<T, DP>(vs + at, PK, g, y);
 #pragma unroll
       for (int k = 0; k < 16; ++k)
-        y[k] *= exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[u][k]) - m, LOG2E, -ll) : exponent<T>(s[k], c, m) - ll);
+        y[k] *= exp2_fast(BIAS ? fmaf(fmaf(s[k], c, bs[u][k]) - m, LOG2E, -ll)
+                               : M::SPLIT ? exponent<T>(s[k], c, m) - ll : fmaf(s[k], c, -m_ll));
       if (t + 1 < t1) fetch_bias(t + 1, u);
       if (word_u != 0xffffffffu) {
 #pragma unroll
@@ -299,12 +301,20 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
 template <typename T, int DP>
 constexpr bool keys_in_lds() { return DP == 128 || (Mma<T>::SPLIT && DP == 64); }
 
+// 128 channels of 16 bits: half of the values as well, and one buffer, so that 80 KB of LDS and 256
+// registers hold a workgroup without spilling (a reload waits for every load before it: 230 -> 185 us at
+// 8192 rows x 2048 keys, 2 x 4 key heads).
+template <typename T, int DP>
+constexpr int dkv_buffers() { return DP == 128 ? 1 : buffers<T, false>(); }
+template <typename T, int DP>
+constexpr int v_steps() { return DP == 128 && !Mma<T>::SPLIT ? 4 : DP / 16; }
+
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void xa_dkv_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::row_stride(DP);
   typedef typename M::L L;
-  constexpr int PT = RT * S, STATS = 3 * RT * 2, NBUF = buffers<T, false>(), BUF = 2 * M::PARTS * PT + STATS;
+  constexpr int PT = RT * S, STATS = 3 * RT * 2, NBUF = dkv_buffers<T, DP>(), BUF = 2 * M::PARTS * PT + STATS;
   constexpr bool KLDS = keys_in_lds<T, DP>();
   extern __shared__ __align__(16) char smem[];
   L* const buf0 = reinterpret_cast<L*>(smem);   // per buffer: q, do, then fp32 [3][RT] maximum, log2 of the sum, delta
@@ -330,7 +340,15 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
       for (int k = 0; k < M::PARTS; ++k) *reinterpret_cast<typename M::part_t*>(kl_at(s) + k * XA_KEYS * KLS) = kf.f[s].p[k];
   }
+  constexpr int VST = v_steps<T, DP>(), VLS = DP - 16 * VST + 8;
+  L* const vl_row = kl + (KLDS ? M::PARTS * XA_KEYS * KLS : 0) + (32 * wid + n) * VLS + 8 * h;
+  if constexpr (VST < DP / 16) {
+#pragma unroll
+    for (int s = VST; s < DP / 16; ++s) *reinterpret_cast<typename M::part_t*>(vl_row + 16 * (s - VST)) = vf.f[s].p[0];
+  }
   const float sf = SCALED<T> ? ds_scale(p, b, hk) : 1.f;
+  // 16-bit types without a bias: maximum and log2 of the sum as one (2^-24 of the logit is nothing there)
+  constexpr bool ONE_STAT = !BIAS && !M::SPLIT;
   constexpr float P_UP = SCALED<T> ? 15.f : 0.f, P_FACTOR = SCALED<T> ? 32768.f : 1.f;
   const float ds_f = sf / P_FACTOR;
   const bool any_seen = __any(seen), all_seen = __all(seen);
@@ -355,7 +373,13 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
     }
     if (sw < 3) {
       stat = sw == 1 ? INFINITY : 0.f;   // a row behind the last: P = 0
-      if (sr < left) stat = (sw == 0 ? p.st_m : sw == 1 ? p.st_l : p.delta)[((long)b * p.H + head) * p.Lq + i0 + sr];
+      const long at = ((long)b * p.H + head) * p.Lq + i0 + sr;
+      if constexpr (ONE_STAT) {
+        if (sw == 0) stat = sr < left ? p.st_m[at] + (p.st_l[at] - P_UP) : INFINITY;
+        else if (sw == 2 && sr < left) stat = p.delta[at];
+      } else if (sr < left) {
+        stat = (sw == 0 ? p.st_m : sw == 1 ? p.st_l : p.delta)[at];
+      }
     }
   };
   auto store_tile = [&](int t) __attribute__((always_inline)) {
@@ -411,20 +435,14 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
         }
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(st + 2 * RT + 32 * u + 8 * run + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dp[4 * run + e] = -dl[e];
-        }
-        dp = inner<T, DP>(gs + at, PT, vf, dp);
-#pragma unroll
-        for (int run = 0; run < 4; ++run) {
           const f32x4 m = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * run + 4 * h);
-          const f32x4 ll = *reinterpret_cast<const f32x4*>(st + RT + 32 * u + 8 * run + 4 * h);
+          f32x4 ll = {};
+          if constexpr (!ONE_STAT) ll = *reinterpret_cast<const f32x4*>(st + RT + 32 * u + 8 * run + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = 4 * run + e;
             pr[k] = exp2_fast(BIAS ? fmaf(fmaf(pr[k], c, bs[u][k]) - m[e], LOG2E, P_UP - ll[e])
-                                   : exponent<T>(pr[k], c, m[e]) + (P_UP - ll[e]));
+                                   : ONE_STAT ? fmaf(pr[k], c, -m[e]) : exponent<T>(pr[k], c, m[e]) - ll[e]);
           }
         }
         if (t + 1 < t1) fetch_bias(t + 1, u);
@@ -432,12 +450,22 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
           for (int k = 0; k < 16; ++k) pr[k] = seen ? pr[k] : 0.f;
         }
+        const typename M::Packed pv[1] = {M::pack(pr)};
+                M::template outer<DT, 1>(gs + 32 * u * S, PT, S, lane, pv, dv);
+        #pragma unroll
+        for (int run = 0; run < 4; ++run) {
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(st + 2 * RT + 32 * u + 8 * run + 4 * h);
 #pragma unroll
+          for (int e = 0; e < 4; ++e) dp[4 * run + e] = -dl[e];
+        }
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+          dp = M::mma(M::load(gs + at + 16 * s, PT), s < VST ? vf.f[s] : M::load(vl_row + 16 * (s - VST), 0), dp);
+        #pragma unroll
         for (int k = 0; k < 16; ++k) dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
-        const typename M::Packed pv[1] = {M::pack(pr)}, pd[1] = {M::pack(dp)};
-        M::template outer<DT, 1>(gs + 32 * u * S, PT, S, lane, pv, dv);
+        const typename M::Packed pd[1] = {M::pack(dp)};
         M::template outer<DT, 1>(qs + 32 * u * S, PT, S, lane, pd, dk);
-      }
+              }
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) store_tile(t + 1);
@@ -545,8 +573,9 @@ int dq_type(const XaParams& p, hipStream_t st) {
 template <typename T, int DP, bool BIAS>
 int dkv_launch(const XaParams& p, hipStream_t st) {
   constexpr int RT = xa_rt(DP, __is_same(T, float)), S = Mma<T>::row_stride(DP);
-  const size_t lds = buffers<T, false>() * ((size_t)4 * Mma<T>::PARTS * RT * S + 3 * RT * 4) +
-                     (keys_in_lds<T, DP>() ? (size_t)2 * Mma<T>::PARTS * XA_KEYS * (Mma<T>::SPLIT ? DP : S) : 0);
+  const size_t lds = dkv_buffers<T, DP>() * ((size_t)4 * Mma<T>::PARTS * RT * S + 3 * RT * 4) +
+                     (keys_in_lds<T, DP>() ? (size_t)2 * Mma<T>::PARTS * XA_KEYS * (Mma<T>::SPLIT ? DP : S) : 0) +
+                     (v_steps<T, DP>() < DP / 16 ? (size_t)2 * XA_KEYS * (DP - 16 * v_steps<T, DP>() + 8) : 0);
   if (int rc = pf_reserve_lds((const void*)xa_dkv_kernel<T, DP, BIAS>, lds, "xa_dkv_kernel")) return rc;
   const int tiles = (p.Lk + XA_KEYS - 1) / XA_KEYS;
   xa_dkv_kernel<T, DP, BIAS><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
