@@ -562,8 +562,9 @@ int pf_dropout_add_fwd(const pf_dropout_args* args);
  * Scores, softmax and sums are fp32; P (16-bit types) is rounded to dtype for the product with v.
  * For the backward pass, the forward pass keeps stats [2][B][H][Lq] (each row's maximum, and log2 of
  * its sum) and, of 16-bit types, o32, the unrounded o: do_i . o_i loses its meaning next to
- * do_i . v_j where one key has nearly all the weight if o is rounded first.  (With a bias gradient,
- * 16-bit types form sum_j P_ij do_i . v_j instead, and o32 is not read.) */
+ * do_i . v_j where one key has nearly all the weight if o is rounded first.  o32_whole != 0 (16-bit
+ * types with a bias whose gradient will be wanted): P is not rounded for o32 either, which leaves
+ * dbias the accuracy of fp32. */
 typedef struct pf_cross_attn_args {
   int B, Lq, Lk, H, Hk, D;
   int dtype, bias_dtype;
@@ -576,6 +577,7 @@ typedef struct pf_cross_attn_args {
   const int* k_lens;                                       /* [B], or NULL */
   void* o;                /* [B][Lq][H][D] */
   float* o32;             /* the same in fp32, or NULL */
+  int o32_whole;
   float* stats;           /* [2][B][H][Lq], or NULL */
   void* workspace; size_t workspace_bytes;
   void* stream;

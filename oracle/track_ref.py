@@ -114,10 +114,9 @@ def cross_attention_slack(r: dict, dtype: torch.dtype, bias=None) -> dict:
     if "do" in r:
         do, dp, delta, ds = (r[n] for n in ("do", "dp", "delta", "ds"))
         mag = do.abs() @ v.abs().transpose(2, 3)
-        edelta = (do.abs() * (eo + (D + 4) * u * r["o"].transpose(1, 2).abs())).sum(3, keepdim=True)
-        if bias is not None:   # with its gradient, delta is summed from the unrounded P and dP
-            edelta = torch.maximum((p * (rel * dp.abs() + (D + Lk + 4) * u * mag + flush * mag)).sum(3, keepdim=True),
-                                   edelta if dtype == torch.float32 else 0 * edelta)
+        # (with a bias, whose gradient is wanted, o is kept from unrounded P for delta)
+        ed = eo if bias is None else (p * (rel + 2.0 ** -22) + tiny * (p > 0)) @ v.abs()
+        edelta = (do.abs() * (ed + (D + 4) * u * r["o"].transpose(1, 2).abs())).sum(3, keepdim=True)
         eds = p * ((D + 4) * u * (mag + delta.abs()) + edelta) + (rel + 4 * u) * ds.abs() + flush * (mag + delta.abs())
         s["dbias"] = eds
         bound = 2 * do.norm(dim=3).amax(2)[..., None, None] * v.norm(dim=3).amax(2)[..., None, None] if Lk and Lq else 0.0

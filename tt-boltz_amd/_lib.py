@@ -141,7 +141,7 @@ class CrossAttnArgs(ctypes.Structure):
         ("v", c_void_p), ("v_b", c_long), ("v_l", c_long), ("v_h", c_long),
         ("bias", c_void_p), ("bias_b", c_long), ("bias_h", c_long), ("bias_q", c_long), ("bias_k", c_long),
         ("mask", c_void_p), ("mask_b", c_long), ("k_lens", c_void_p),
-        ("o", c_void_p), ("o32", c_void_p), ("stats", c_void_p),
+        ("o", c_void_p), ("o32", c_void_p), ("o32_whole", c_int), ("stats", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("stream", c_void_p),
         ("dout", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dbias", c_void_p),
         ("dbias_B", c_int), ("dbias_H", c_int),

@@ -25,6 +25,7 @@ struct XaParams {
   int splits, per;               // key tiles (dkv: row tiles) per split
   int few;                       // the waves of a workgroup share a 32-row tile
   int wide;                      // forward: two 32-row tiles per wave
+  int whole;                     // forward, 16-bit types with a bias: o32 to fp32's accuracy
   // backward
   const void* dout;              // [B][Lq][H][D]
   float* delta;                  // [B][H][Lq]
@@ -50,5 +51,3 @@ int pf_xa_fwd_bf16(const XaParams& p, hipStream_t st);
 int pf_xa_delta_bf16(const XaParams& p, float* amax, hipStream_t st);
 int pf_xa_dq_bf16(const XaParams& p, hipStream_t st);
 int pf_xa_dkv_bf16(const XaParams& p, hipStream_t st);
-int pf_xa_exact_delta_fp16(const XaParams& p, hipStream_t st);
-int pf_xa_exact_delta_bf16(const XaParams& p, hipStream_t st);

@@ -157,6 +157,7 @@ extern "C" int pf_cross_attn_fwd(const pf_cross_attn_args* a) {
     return pf_fail(PF_E_INVALID, "%s: workspace too small (%zu < %zu bytes)", fn, a->workspace_bytes, need);
   if (need && !pf_aligned16(a->workspace)) return pf_fail(PF_E_INVALID, "%s: workspace not 16-byte aligned", fn);
   p.splits = s.splits, p.per = s.per, p.part = (float*)a->workspace;
+  p.whole = a->o32_whole != 0;
   // Two row tiles per wave (64 channels without a bias: each LDS read serves two products) where
   // workgroups of 256 rows still come to two per CU: 16 heads x 2048 rows x 4096 keys, batch 4 (512
   // workgroups) 185 against 198 us, batch 2 (256) 113 against 109.
@@ -181,8 +182,7 @@ extern "C" int pf_cross_attn_bwd(const pf_cross_attn_args* a) {
                                                             : pf_fail(PF_E_INVALID, "%s: no queries (the caller clears dk and dv)", fn);
   if (int rc = check_data(a, fn)) return rc;
   const float* o32 = a->dtype == PF_FP32 ? (const float*)a->o : a->o32;
-  const bool exact = a->dbias && a->dtype != PF_FP32;   // delta from P and dP themselves
-  if (!a->dout || (!o32 && !exact) || !a->stats) return pf_fail(PF_E_INVALID, "%s: dout, the unrounded o and the statistics are needed", fn);
+  if (!a->dout || !o32 || !a->stats) return pf_fail(PF_E_INVALID, "%s: dout, the unrounded o and the statistics are needed", fn);
   if ((a->dk != nullptr) != (a->dv != nullptr)) return pf_fail(PF_E_INVALID, "%s: dk and dv come together", fn);
   if (a->dbias && !a->dq) return pf_fail(PF_E_INVALID, "%s: dbias comes with dq", fn);
   if (!pf_aligned16(a->dout) || !pf_aligned16(o32) || !pf_aligned16(a->dq) || !pf_aligned16(a->dk) || !pf_aligned16(a->dv) ||
@@ -202,20 +202,9 @@ extern "C" int pf_cross_attn_bwd(const pf_cross_attn_args* a) {
   p.dout = a->dout, p.amax = amax, p.part = (float*)(ws + l.part);
   p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
   const int t = a->dtype;
-  p.delta = exact ? nullptr : delta;
-  if (int rc = t == PF_FP32   ? pf_xa_delta_fp32(p, amax, st)
-               : t == PF_FP16 ? pf_xa_delta_fp16(p, amax, st)
-               : exact        ? PF_OK
-                              : pf_xa_delta_bf16(p, amax, st))
-    return rc;
   p.delta = delta;
-  if (exact) {
-    const Split s = key_split(p, a->dtype);
-    XaParams d = p;
-    d.splits = s.splits, d.per = s.per;
-    if (s.splits == 1) d.part = delta;
-    if (int rc = t == PF_FP16 ? pf_xa_exact_delta_fp16(d, st) : pf_xa_exact_delta_bf16(d, st)) return rc;
-  }
+  if (int rc = t == PF_FP32 ? pf_xa_delta_fp32(p, amax, st) : t == PF_FP16 ? pf_xa_delta_fp16(p, amax, st) : pf_xa_delta_bf16(p, amax, st))
+    return rc;
   if (a->dq) {
     const Split s = key_split(p, a->dtype);
     XaParams d = p;

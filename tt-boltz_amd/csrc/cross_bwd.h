@@ -30,7 +30,7 @@ PF_DEV float ds_scale(const XaParams& p, int b, int hk) {
 }
 
 // ------------------------------------------------------------------------------ delta
-// delta_i = do_i . o_i in fp32 from the unrounded o (p.delta null: not wanted), 8 lanes a row; fp16:
+// delta_i = do_i . o_i in fp32 from the unrounded o, 8 lanes a row; fp16:
 // also the largest |do_i|^2 and |v_j|^2 of the workgroup's part of a key head (ds_scale joins the parts).
 // blockIdx.x: the part (at most 64), blockIdx.y: batch element and key head.
 template <typename T>
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
     for (int d = 4 * sub; d < p.D; d += 32) {
       typedef T quad __attribute__((ext_vector_type(4)));
       const quad g4 = *reinterpret_cast<const quad*>((const T*)p.dout + at + d);
-      const f32x4 o4 = p.delta ? *reinterpret_cast<const f32x4*>(o32 + at + d) : (f32x4)(0.f);
+      const f32x4 o4 = *reinterpret_cast<const f32x4*>(o32 + at + d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         dot = fmaf((float)g4[e], o4[e], dot);
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
       dot += __shfl_xor(dot, o);
       sq += __shfl_xor(sq, o);
     }
-    if (sub == 0 && p.delta) p.delta[(b * p.H + head) * p.Lq + i] = dot;
+    if (sub == 0) p.delta[(b * p.H + head) * p.Lq + i] = dot;
     g_top = fmaxf(g_top, sq);
   }
   if constexpr (SCALED<T>) {
@@ -92,16 +92,13 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
 }
 
 // ------------------------------------------------------------------------------ dq, dS
-// DELTA: delta_i = sum_j P_ij (do_i . v_j) instead, of the split's keys, from the fp32 P and dP that dS will
-// be made of.  A bias's gradient is dS itself, in fp32 as a rule, and do . o is not good enough for it:
-// 16-bit types round P in o's product (2^-9 or 2^-12 of delta, against 2^-22 here).
 template <typename T, int DP, bool BIAS, bool FEW>
 constexpr int dq_waves() {
   if (DP == 128) return FEW || __is_same(T, float) ? 1 : 2;
   return __is_same(T, float) || DP == 64 || BIAS ? 2 : FEW ? 3 : 4;
 }
 
-template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
+template <typename T, int DP, bool BIAS, bool FEW>
 __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
@@ -125,15 +122,14 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
   const long stat = ((long)b * p.H + head) * p.Lq + i;
   const float m = row_ok ? p.st_m[stat] : 0.f, ll = row_ok ? p.st_l[stat] : INFINITY;
   const float m_ll = m + ll;   // 16-bit types without a bias (2^-24 of the logit is nothing there)
-  const float delta = !DELTA && row_ok ? p.delta[stat] : 0.f;
-  const float sf = SCALED<T> && !DELTA ? ds_scale(p, b, hk) : 1.f;
-  float sum = 0.f;   // DELTA: this lane's half of the keys
+  const float delta = row_ok ? p.delta[stat] : 0.f;
+  const float sf = SCALED<T> ? ds_scale(p, b, hk) : 1.f;
   const char* bias = nullptr;
   if constexpr (BIAS) bias = bias_row<T>(p, b, head, i);
-  float* const ds = !DELTA && p.ds && row_ok ? p.ds + stat * p.Lk : nullptr;
+  float* const ds = p.ds && row_ok ? p.ds + stat * p.Lk : nullptr;
   const int len = length_of(p, b);
   // the logits' gradient has zeros at hidden keys, so its writer goes on to the end
-  const int t0 = blk.z * p.per, t1 = min(t0 + p.per, ((!DELTA && p.ds ? p.Lk : len) + KT - 1) / KT);
+  const int t0 = blk.z * p.per, t1 = min(t0 + p.per, ((p.ds ? p.Lk : len) + KT - 1) / KT);
   const uint8_t* mask = p.mask ? p.mask + b * p.mb : nullptr;
   const T* const kb = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* const vb = (const T*)p.v + b * p.vb + hk * p.vh;
@@ -176,7 +172,7 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
       const uint32_t word_u = (uint32_t)(word >> (FEW ? 0 : 32 * u));
-      if (!word_u && (DELTA || !p.ds)) {
+      if (!word_u && !p.ds) {
         if (t + 1 < t1) fetch_bias(t + 1, u);
         continue;
       }
@@ -195,11 +191,6 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
       if (word_u != 0xffffffffu) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) y[k] = (word_u >> (4 * h) >> acc_row(k, 0)) & 1 ? y[k] : 0.f;
-      }
-      if constexpr (DELTA) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) sum += y[k];
-        continue;
       }
       if (ds) {
 #pragma unroll
@@ -234,19 +225,6 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
     __syncthreads();
   }
 
-  if constexpr (DELTA) {
-    sum = xor32_sum(sum);
-    float* const to = p.part + (long)blk.z * p.B * p.H * p.Lq;
-    if constexpr (FEW) {
-      float* const part = reinterpret_cast<float*>(smem);   // [4][32]
-      if (h == 0) part[32 * wid + n] = sum;
-      __syncthreads();
-      if (threadIdx.x < 32 && row_ok) to[stat] = part[n] + part[32 + n] + part[64 + n] + part[96 + n];
-    } else if (h == 0 && row_ok) {
-      to[stat] = sum;
-    }
-    return;
-  }
   const float out_scale = p.grad_scale / sf;
   if constexpr (FEW) {
     constexpr int OS = DP + 4;
@@ -507,13 +485,6 @@ __global__ __launch_bounds__(256) void xa_sum_kernel(const float* __restrict__ p
   const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (e >= n) return;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
-  if (e + 3 >= n || step % 4) {   // statistics: any number of rows
-    for (int k = 0; k < 4 && e + k < n; ++k) {
-      for (int z = 0; z < splits; ++z) a[k] += part[z * step + e + k];
-      out[e + k] = (T)a[k];
-    }
-    return;
-  }
 #pragma unroll 4
   for (int z = 0; z < splits; ++z) {
     const f32x4 v = *reinterpret_cast<const f32x4*>(part + z * step + e);
@@ -530,44 +501,30 @@ int sum_launch(const float* part, long step, int splits, void* out0, void* out1,
   return PF_OK;
 }
 
-template <typename T, int DP, bool BIAS, bool FEW, bool DELTA>
+template <typename T, int DP, bool BIAS, bool FEW>
 int dq_launch(const XaParams& p, hipStream_t st) {
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
-  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * 2 * Mma<T>::PARTS * buffers<T, FEW>(), join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0;
-  const size_t lds = tiles > join ? tiles : join;
-  if (int rc = pf_reserve_lds((const void*)xa_dq_kernel<T, DP, BIAS, FEW, DELTA>, lds, "xa_dq_kernel")) return rc;
+  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * 2 * Mma<T>::PARTS * buffers<T, FEW>(),
+               join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0, lds = tiles > join ? tiles : join;
+  if (int rc = pf_reserve_lds((const void*)xa_dq_kernel<T, DP, BIAS, FEW>, lds, "xa_dq_kernel")) return rc;
   const int rt = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
-  xa_dq_kernel<T, DP, BIAS, FEW, DELTA><<<(unsigned)((long)rt * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
+  xa_dq_kernel<T, DP, BIAS, FEW><<<(unsigned)((long)rt * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
   PF_CHECK_LAUNCH("xa_dq_kernel");
-  if (p.splits == 1) return PF_OK;
-  const long rows = (long)p.B * p.Lq * p.H;
-  return DELTA ? sum_launch<float>(p.part, rows, p.splits, p.delta, nullptr, rows, st)
-               : sum_launch<T>(p.part, rows * p.D, p.splits, p.dq, nullptr, rows * p.D, st);
+  const long n = (long)p.B * p.Lq * p.H * p.D;
+  return p.splits > 1 ? sum_launch<T>(p.part, n, p.splits, p.dq, nullptr, n, st) : PF_OK;
 }
 
-template <typename T, int DP, bool DELTA>
+template <typename T, int DP>
 int dq_dp(const XaParams& p, hipStream_t st) {
   if constexpr (has_few<T, DP>()) {
-    if (p.few && p.bias) return dq_launch<T, DP, true, true, DELTA>(p, st);
-    if constexpr (!DELTA) {
-      if (p.few) return dq_launch<T, DP, false, true, false>(p, st);
-    }
+    if (p.few) return p.bias ? dq_launch<T, DP, true, true>(p, st) : dq_launch<T, DP, false, true>(p, st);
   }
-  if constexpr (!DELTA) {
-    if (!p.bias) return dq_launch<T, DP, false, false, false>(p, st);
-  }
-  return dq_launch<T, DP, true, false, DELTA>(p, st);
-}
-
-// delta of 16-bit types with a bias gradient (part: where the splits go, delta itself if there is one)
-template <typename T>
-int exact_delta_type(const XaParams& p, hipStream_t st) {
-  return p.D <= 32 ? dq_dp<T, 32, true>(p, st) : p.D <= 64 ? dq_dp<T, 64, true>(p, st) : dq_dp<T, 128, true>(p, st);
+  return p.bias ? dq_launch<T, DP, true, false>(p, st) : dq_launch<T, DP, false, false>(p, st);
 }
 
 template <typename T>
 int dq_type(const XaParams& p, hipStream_t st) {
-  return p.D <= 32 ? dq_dp<T, 32, false>(p, st) : p.D <= 64 ? dq_dp<T, 64, false>(p, st) : dq_dp<T, 128, false>(p, st);
+  return p.D <= 32 ? dq_dp<T, 32>(p, st) : p.D <= 64 ? dq_dp<T, 64>(p, st) : dq_dp<T, 128>(p, st);
 }
 
 template <typename T, int DP, bool BIAS>

@@ -122,6 +122,17 @@ struct Mma {
     }
     return b;
   }
+  // 16-bit types: x to fp32's accuracy in WHOLE roundings, each of the rest of the ones before
+  static constexpr int WHOLE = __is_same(T, half_t) ? 2 : 3;
+  static PF_DEV void pack_whole(const f32x16& x, Packed (&b)[WHOLE]) {
+    f32x16 r = x;
+#pragma unroll
+    for (int k = 0; k < WHOLE; ++k) {
+      b[k] = pack(r);
+#pragma unroll
+      for (int t = 0; t < 16; ++t) r[t] -= (float)b[k].f[t >> 3].p[0][t & 7];
+    }
+  }
   // 16-bit types: c + the sum of this lane's 16 values as they were rounded
   static PF_DEV float sum(const Packed& b, float c) {
     typedef L pair_t __attribute__((ext_vector_type(2)));
@@ -162,6 +173,21 @@ struct Mma {
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][dt] = mma(a, p[r].f[s], acc[r][dt]);
+      }
+  }
+  // 16-bit types: acc[dt] += X^T (P[0] + P[1] + ..)
+  template <int DT, int K>
+  static PF_DEV void outer_sum(const L* x, int st, int lane, const Packed (&p)[K], f32x16 (&acc)[DT]) {
+    const int h = lane >> 5, i = lane & 15, c16 = (lane >> 4) & 1;
+    const L* at = x + (4 * h + (i >> 2)) * st + 16 * c16 + 4 * (i & 3);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const quad_t lo = tr_read(at + 32 * dt + (16 * s) * st), hi = tr_read(at + 32 * dt + (16 * s + 8) * st);
+        const part_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) acc[dt] = mma1(a, p[k].f[s].p[0], acc[dt]);
       }
   }
   static PF_DEV quad_t tr_read(const L* p) {
@@ -406,7 +432,10 @@ constexpr int fwd_waves() {
   return __is_same(T, float) ? 2 : DP == 64 ? (BIAS ? 2 : FEW ? 3 : 4) : BIAS && !FEW ? 3 : 4;
 }
 
-template <typename T, int DP, bool BIAS, bool FEW, int R>
+// WHOLE (16-bit types): P enters the product with the values to fp32's accuracy.  A bias's gradient is
+// dS = P (dP - delta) itself, fp32 as a rule, and delta = do . o of an o made from rounded P would leave it
+// with 2^-9 or 2^-12 of delta.
+template <typename T, int DP, bool BIAS, bool FEW, int R, bool WHOLE>
 __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fwd_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
@@ -510,6 +539,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
     if (t + 1 < t1) fetch_bias(t + 1);
     if (word) {
       typename M::Packed pk[NSUB][R];
+      typename M::Packed whole[NSUB][M::WHOLE];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float mx = -INFINITY;
@@ -535,7 +565,8 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
           f32x16 pr;
 #pragma unroll
           for (int k = 0; k < 16; ++k) pr[k] = exp2_fast(BIAS ? (x[u][r][k] - mu) * LOG2E : exponent<T>(x[u][r][k], c, mu));
-          pk[u][r] = M::pack(pr);
+          if constexpr (WHOLE) M::pack_whole(pr, whole[u]);
+          else pk[u][r] = M::pack(pr);
           if constexpr (BIAS || M::SPLIT) {   // a bias's gradient wants P, and so the sum, to fp32
 #pragma unroll
             for (int k = 0; k < 16; ++k) l[r] += pr[k];
@@ -545,7 +576,10 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fw
         }
       }
 #pragma unroll
-      for (int u = 0; u < NSUB; ++u) M::template outer<DT, R>(vs + (sub0 + 32 * u) * VS, PV, VS, lane, pk[u], o);
+      for (int u = 0; u < NSUB; ++u) {
+        if constexpr (WHOLE) M::template outer_sum<DT, M::WHOLE>(vs + (sub0 + 32 * u) * VS, VS, lane, whole[u], o[0]);
+        else M::template outer<DT, R>(vs + (sub0 + 32 * u) * VS, PV, VS, lane, pk[u], o);
+      }
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) {
@@ -700,13 +734,14 @@ size_t fwd_lds() {
   return tiles > join ? tiles : join;
 }
 
-template <typename T, int DP, bool BIAS, bool FEW, int R>
+template <typename T, int DP, bool BIAS, bool FEW, int R, bool WHOLE = false>
 int fwd_launch(const XaParams& p, hipStream_t st) {
   const size_t lds = fwd_lds<T, DP, FEW>();
-  if (int rc = pf_reserve_lds((const void*)xa_fwd_kernel<T, DP, BIAS, FEW, R>, lds, "xa_fwd_kernel")) return rc;
+  const auto kernel = xa_fwd_kernel<T, DP, BIAS, FEW, R, WHOLE>;
+  if (int rc = pf_reserve_lds((const void*)kernel, lds, "xa_fwd_kernel")) return rc;
   constexpr int ROWS = FEW ? 32 : 128 * R;
   const int tiles = (p.rows + ROWS - 1) / ROWS;
-  xa_fwd_kernel<T, DP, BIAS, FEW, R><<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
+  kernel<<<(unsigned)((long)tiles * p.splits * p.B * p.Hk), 256, lds, st>>>(p);
   PF_CHECK_LAUNCH("xa_fwd_kernel");
   if (p.splits > 1) {
     const long threads = (long)p.B * p.Hk * p.rows * (p.D / 4);
@@ -722,6 +757,9 @@ constexpr bool has_few() { return !(Mma<T>::SPLIT && DP == 128); }
 
 template <typename T, int DP>
 int fwd_dp(const XaParams& p, hipStream_t st) {
+  if constexpr (!Mma<T>::SPLIT) {
+    if (p.bias && p.whole) return p.few ? fwd_launch<T, DP, true, true, 1, true>(p, st) : fwd_launch<T, DP, true, false, 1, true>(p, st);
+  }
   if constexpr (has_few<T, DP>()) {
     if (p.few) return p.bias ? fwd_launch<T, DP, true, true, 1>(p, st) : fwd_launch<T, DP, false, true, 1>(p, st);
   }

@@ -100,7 +100,7 @@ def _strides(t: torch.Tensor) -> tuple:
     return s[:3]
 
 
-def _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats) -> "_lib.CrossAttnArgs":
+def _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats, whole=0) -> "_lib.CrossAttnArgs":
     (B, Lq, H, D), (_, Lk, Hk, _) = q.shape, k.shape
     if bias is None:
         bias_code, bias_at, bias_strides = 0, None, (0, 0, 0, 0)
@@ -110,7 +110,7 @@ def _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats) -> "_lib.Cros
     return _lib.CrossAttnArgs(
         B, Lq, Lk, H, Hk, D, DTYPE_CODE[q.dtype], bias_code, scale, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k),
         v.data_ptr(), *_strides(v), bias_at, *bias_strides, None if mask is None else mask.data_ptr(),
-        0 if mask is None or B == 1 else mask.stride(0), ops._ptr(k_lens), ops._ptr(o), ops._ptr(o32), ops._ptr(stats),
+        0 if mask is None or B == 1 else mask.stride(0), ops._ptr(k_lens), ops._ptr(o), ops._ptr(o32), whole, ops._ptr(stats),
         None, 0, ops._stream())
 
 
@@ -128,12 +128,13 @@ def launch_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o:
                            bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                            k_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                            o32: Optional[torch.Tensor] = None, stats: Optional[torch.Tensor] = None,
-                           ws: Optional[torch.Tensor] = None) -> None:
+                           ws: Optional[torch.Tensor] = None, o32_whole: bool = False) -> None:
     """o = cross attention (pf_cross_attn_fwd) of q [B, Lq, H, D] on k, v [B, Lk, Hk, D]; bias
     [B or 1, H or 1, Lq, Lk], mask bool or uint8 [B, Lk], k_lens int32 [B].  ``o32`` fp32 like o (16-bit
     types) and ``stats`` fp32 [2, B, H, Lq] keep what the backward pass needs; ``ws`` of
-    ``cross_attention_workspace_bytes``.  (With a bias gradient, 16-bit types need no ``o32``.)"""
-    a = _cross_args(q, k, v, bias, mask, k_lens, q.shape[-1] ** -0.5 if scale is None else scale, o, o32, stats)
+    ``cross_attention_workspace_bytes``.  ``o32_whole``: o32 from unrounded probabilities, for a bias's gradient."""
+    a = _cross_args(q, k, v, bias, mask, k_lens, q.shape[-1] ** -0.5 if scale is None else scale, o, o32, stats,
+                    int(o32_whole))
     if ws is not None:
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _lib.check(_lib.load().pf_cross_attn_fwd(ctypes.byref(a)), "pf_cross_attn_fwd")
@@ -173,17 +174,17 @@ def launch_cross_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     _lib.check(_lib.load().pf_cross_attn_bwd(ctypes.byref(a)), "pf_cross_attn_bwd")
 
 
-def _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep: bool, keep_o: bool):
+def _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep: bool, whole: bool):
     """(o, o32, stats) on strided tensors; the last two only where a backward pass will read them."""
     dev = q.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep, keep_o)
+            return _cross_fwd(q, k, v, bias, mask, k_lens, scale, keep, whole)
     shape = q.shape
     o = torch.empty(shape, dtype=q.dtype, device=dev)
-    o32 = torch.empty(shape, dtype=torch.float32, device=dev) if keep_o and q.dtype != torch.float32 else None
+    o32 = torch.empty(shape, dtype=torch.float32, device=dev) if keep and q.dtype != torch.float32 else None
     stats = torch.empty((2, shape[0], shape[2], shape[1]), dtype=torch.float32, device=dev) if keep else None
-    a = _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats)
+    a = _cross_args(q, k, v, bias, mask, k_lens, scale, o, o32, stats, int(whole))
     ws = _with_workspace(a, "pf_cross_attn_workspace_size", dev)  # noqa: F841
     _lib.check(_lib.load().pf_cross_attn_fwd(ctypes.byref(a)), "pf_cross_attn_fwd")
     return o, o32, stats
@@ -211,8 +212,7 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, mask, k_lens, scale):
         q, k, v = _strided(q), _strided(k), _strided(v)
-        # (a bias gradient of 16-bit types does without the unrounded o)
-        o, o32, stats = _cross_fwd(q, k, v, bias, mask, k_lens, scale, True, not ctx.needs_input_grad[3])
+        o, o32, stats = _cross_fwd(q, k, v, bias, mask, k_lens, scale, True, ctx.needs_input_grad[3])
         ctx.save_for_backward(q, k, v, bias, mask, k_lens, o if q.dtype == torch.float32 else o32, stats)
         ctx.scale = scale
         return o
