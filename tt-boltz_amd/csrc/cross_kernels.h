@@ -425,8 +425,9 @@ template <typename T, bool FEW>
 constexpr int buffers() { return FEW || __is_same(T, float) ? 1 : 2; }
 
 // Waves per SIMD that the forward kernel's registers are kept to.
-template <typename T, int DP, bool BIAS, bool FEW, int R>
+template <typename T, int DP, bool BIAS, bool FEW, int R, bool WHOLE>
 constexpr int fwd_waves() {
+  if (WHOLE && DP <= 64) return FEW && DP == 32 ? 3 : 2;
   if (DP == 128) return FEW || __is_same(T, float) ? 1 : 2;
   if (R == 2) return 2;
   return __is_same(T, float) ? 2 : DP == 64 ? (BIAS ? 2 : FEW ? 3 : 4) : BIAS && !FEW ? 3 : 4;
@@ -436,7 +437,7 @@ constexpr int fwd_waves() {
 // dS = P (dP - delta) itself, fp32 as a rule, and delta = do . o of an o made from rounded P would leave it
 // with 2^-9 or 2^-12 of delta.
 template <typename T, int DP, bool BIAS, bool FEW, int R, bool WHOLE>
-__global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R>())) void xa_fwd_kernel(XaParams p) {
+__global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R, WHOLE>())) void xa_fwd_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
   constexpr int KS = M::row_stride(DP), VS = M::col_stride(DP);
