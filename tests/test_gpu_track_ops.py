@@ -503,6 +503,14 @@ def test_cross_attention_offsets_past_32_bits(gpu):
     buf = torch.empty(2 ** 32 + 2 ** 21, dtype=torch.float16, device=gpu)
     k = buf.as_strided((2, 70, 2, 32), (2 ** 31, 64, 32, 1))
     v = buf.as_strided((2, 70, 2, 32), (2 ** 20, 64, 2 ** 32, 1), 8192)
+    far = buf.as_strided((2, 2040, 2, 32), (32, 2 ** 21, 64, 1))   # rows 2^21 elements apart
+    far.copy_(torch.randn(far.shape, device=gpu))
+    q = far[:, -40:]
+    near = far.contiguous()
+    p = ops.cross_attention(q.detach().contiguous().requires_grad_(), near.requires_grad_(), near)
+    o = ops.cross_attention(q.detach().requires_grad_(), far.requires_grad_(), far)
+    assert torch.equal(o, p)
+    assert torch.equal(torch.autograd.grad(o, far, torch.ones_like(o))[0], torch.autograd.grad(p, near, torch.ones_like(p))[0])
     k.copy_(torch.randn(k.shape, device=gpu)), v.copy_(torch.randn(v.shape, device=gpu))
     for Lq in (1, 50):
         q, do = torch.randn((2, Lq, 4, 32), device=gpu).half().requires_grad_(), torch.randn((2, Lq, 4, 32), device=gpu).half()

@@ -101,12 +101,16 @@ BwdLayout bwd_layout(const pf_cross_attn_args* a, const XaParams& p) {
   return l;
 }
 
-bool grid_fits(const XaParams& p) {   // a launch holds fewer than 2^32 threads
-  const long rt = ((long)p.Lq + 31) / 32 * p.G, kt = ((long)p.Lk + XA_KEYS - 1) / XA_KEYS;
-  const long most = (rt > kt ? rt : kt) * p.B;
-  if (most >= (1l << 24) || most * p.Hk >= (1l << 24) || (long)p.B * p.Hk > 65535) return false;
-  const long q = (long)p.B * p.Lq * p.H, k = (long)p.B * p.Lk * p.Hk;   // rows: 8 threads each, or one for 4 channels
-  return q + k < (1l << 29) && q * p.D < (1l << 34) && k * p.D < (1l << 34);
+// A launch holds fewer than 2^32 threads: 2^24 workgroups (splits are made where there are few), and
+// element-wise launches of a thread for four channels.
+bool grid_fits(const XaParams& p, bool backward) {
+  const long rt = ((long)p.rows + (p.few ? 31 : 127)) / (p.few ? 32 : 128);
+  const long kt = backward ? ((long)p.Lk + XA_KEYS - 1) / XA_KEYS : 0, chunks = backward ? p.chunks : 0;
+  long most = rt > kt ? rt : kt;
+  if (chunks > most) most = chunks;
+  if (most >= 1l << 24 || most * p.B >= 1l << 24 || most * p.B * p.Hk >= 1l << 24) return false;
+  const long q = (long)p.B * p.Lq * p.H, k = (long)p.B * p.Lk * p.Hk;
+  return q < 1l << 31 && k < 1l << 31 && q * p.D < 1l << 34 && k * p.D < 1l << 34;
 }
 
 // dbias[bb, hh, e] = sum of ds[b, h, e] over the dimensions of size 1, e < Lq Lk: lanes on neighbouring
@@ -150,7 +154,7 @@ extern "C" int pf_cross_attn_fwd(const pf_cross_attn_args* a) {
   if (!a->o) return pf_fail(PF_E_INVALID, "%s: null pointer", fn);
   if (!pf_aligned16(a->o) || !pf_aligned16(a->o32)) return pf_fail(PF_E_INVALID, "%s: o must be 16-byte aligned", fn);
   XaParams p = params_of(a);
-  if (!grid_fits(p)) return pf_fail(PF_E_INVALID, "%s: too large (B=%d Lq=%d Lk=%d H=%d)", fn, a->B, a->Lq, a->Lk, a->H);
+  if (!grid_fits(p, false)) return pf_fail(PF_E_INVALID, "%s: too large (B=%d Lq=%d Lk=%d H=%d)", fn, a->B, a->Lq, a->Lk, a->H);
   const Split s = key_split(p, a->dtype);
   const size_t need = (size_t)fwd_part_bytes(p, s);
   if (need && (!a->workspace || a->workspace_bytes < need))
@@ -189,7 +193,7 @@ extern "C" int pf_cross_attn_bwd(const pf_cross_attn_args* a) {
       !pf_aligned16(a->dbias) || !pf_aligned16(a->workspace))
     return pf_fail(PF_E_INVALID, "%s: gradients and workspace must be 16-byte aligned", fn);
   XaParams p = params_of(a);
-  if (!grid_fits(p)) return pf_fail(PF_E_INVALID, "%s: too large (B=%d Lq=%d Lk=%d H=%d)", fn, a->B, a->Lq, a->Lk, a->H);
+  if (!grid_fits(p, true)) return pf_fail(PF_E_INVALID, "%s: too large (B=%d Lq=%d Lk=%d H=%d)", fn, a->B, a->Lq, a->Lk, a->H);
   if (a->dbias && (((long)a->Lq * a->Lk) >> 32 || (long)a->dbias_B * a->dbias_H > 65535))
     return pf_fail(PF_E_INVALID, "%s: bias gradient too large (Lq=%d Lk=%d B=%d H=%d)", fn, a->Lq, a->Lk, a->dbias_B, a->dbias_H);
   const BwdLayout l = bwd_layout(a, p);

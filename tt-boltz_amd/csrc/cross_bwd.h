@@ -32,16 +32,16 @@ PF_DEV float ds_scale(const XaParams& p, int b, int hk) {
 // ------------------------------------------------------------------------------ delta
 // delta_i = do_i . o_i in fp32 from the unrounded o, 8 lanes a row; fp16:
 // also the largest |do_i|^2 and |v_j|^2 of the workgroup's part of a key head (ds_scale joins the parts).
-// blockIdx.x: the part (at most 64), blockIdx.y: batch element and key head.
+// blockIdx.x: batch element and key head, and its part (at most 64).
 template <typename T>
 __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __restrict__ amax) {
   __shared__ float top[2][4];
   const int sub = threadIdx.x & 7;
-  const long b = blockIdx.y / p.Hk;
-  const int hk = blockIdx.y % p.Hk;
+  const int bh = blockIdx.x / p.chunks, chunk = blockIdx.x - bh * p.chunks, hk = bh % p.Hk;
+  const long b = bh / p.Hk;
   const float* o32 = p.o32 ? p.o32 : (const float*)p.o;
   float g_top = 0.f, v_top = 0.f;
-  for (int r = blockIdx.x * 32 + (threadIdx.x >> 3); r < p.rows; r += 32 * gridDim.x) {
+  for (int r = chunk * 32 + (threadIdx.x >> 3); r < p.rows; r += 32 * p.chunks) {
     const int i = r / p.G, head = hk * p.G + r - i * p.G;
     const long at = ((b * p.Lq + i) * p.H + head) * p.D;
     float dot = 0.f, sq = 0.f;
@@ -65,10 +65,10 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
   }
   if constexpr (SCALED<T>) {
     const int len = length_of(p, (int)b);
-    for (int key = blockIdx.x * 32 + (threadIdx.x >> 3); key < len; key += 32 * gridDim.x) {
+    for (int key = chunk * 32 + (threadIdx.x >> 3); key < len; key += 32 * p.chunks) {
       float sq = 0.f;
       if (!p.mask || p.mask[b * p.mb + key]) {
-        const T* v = (const T*)p.v + b * p.vb + key * p.vl + hk * p.vh;
+        const T* v = (const T*)p.v + b * p.vb + (long)key * p.vl + hk * p.vh;
         for (int d = 4 * sub; d < p.D; d += 32) {
           typedef T quad __attribute__((ext_vector_type(4)));
           const quad v4 = *reinterpret_cast<const quad*>(v + d);
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void xa_delta_kernel(XaParams p, float* __rest
     __syncthreads();
     if (threadIdx.x < 2) {
       const float* t = top[threadIdx.x];
-      amax[((long)blockIdx.y * gridDim.x + blockIdx.x) * 2 + threadIdx.x] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      amax[(long)blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
     }
   }
 }
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_ker
   const int sub0 = FEW ? 32 * wid : 0;
   const long row_at = ((long)b * p.Lq + i) * p.H + head;
   Frag<T, DP> q, g;
-  q.load((const T*)p.q + b * p.qb + i * p.ql + head * p.qh, p.D, h, row_ok, p.neg);
+  q.load((const T*)p.q + b * p.qb + (long)i * p.ql + head * p.qh, p.D, h, row_ok, p.neg);
   g.load((const T*)p.dout + row_at * p.D, p.D, h, row_ok);
   const long stat = ((long)b * p.H + head) * p.Lq + i;
   const float m = row_ok ? p.st_m[stat] : 0.f, ll = row_ok ? p.st_l[stat] : INFINITY;
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
   const int sw = threadIdx.x / RT, sr = threadIdx.x % RT;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
     const int g = t / head_tiles, i0 = (t - g * head_tiles) * RT, head = hk * p.G + g, left = p.Lq - i0;
-    const T* qp = (const T*)p.q + b * p.qb + i0 * p.ql + head * p.qh;
+    const T* qp = (const T*)p.q + b * p.qb + (long)i0 * p.ql + head * p.qh;
     const T* gp = (const T*)p.dout + (((long)b * p.Lq + i0) * p.H + head) * p.D;
     if (left >= RT) {
       sq.load(qp, p.ql, p.D);
@@ -554,7 +554,7 @@ int dkv_type(const XaParams& p, hipStream_t st) {
 
 template <typename T>
 int delta_type(const XaParams& p, float* amax, hipStream_t st) {
-  xa_delta_kernel<T><<<dim3((unsigned)p.chunks, (unsigned)(p.B * p.Hk)), 256, 0, st>>>(p, amax);
+  xa_delta_kernel<T><<<(unsigned)((long)p.chunks * p.B * p.Hk), 256, 0, st>>>(p, amax);
   PF_CHECK_LAUNCH("xa_delta_kernel");
   return PF_OK;
 }

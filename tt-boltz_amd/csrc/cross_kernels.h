@@ -255,7 +255,7 @@ struct Stage {
   static PF_DEV int row(int j) { return (int)threadIdx.x / PER + j * STEP; }
   static PF_DEV int chan() { return (int)threadIdx.x % PER * N; }
   // this thread's first piece, in bytes from the tile's first row (row strides are below 2^22 elements)
-  static PF_DEV uint32_t first(int stride) { return (uint32_t)((row(0) * stride + chan()) * (int)sizeof(T)); }
+  static PF_DEV uint32_t first(int stride) { return ((uint32_t)row(0) * (uint32_t)stride + (uint32_t)chan()) * (uint32_t)sizeof(T); }
   // p: row 0 of the tile, rows `stride` apart; all rows are there
   PF_DEV void load(const T* p, int stride, int D) {
     if (chan() < D) {
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R, WHOLE>())) voi
     row_ok[r] = row[r] < p.rows;
     i[r] = row_ok[r] ? row[r] / p.G : 0;
     head[r] = hk * p.G + (row_ok[r] ? row[r] - i[r] * p.G : 0);
-    q[r].load((const T*)p.q + b * p.qb + i[r] * p.ql + head[r] * p.qh, p.D, h, row_ok[r], p.neg);
+    q[r].load((const T*)p.q + b * p.qb + (long)i[r] * p.ql + head[r] * p.qh, p.D, h, row_ok[r], p.neg);
     if constexpr (BIAS) bias[r] = bias_row<T>(p, b, head[r], i[r]);
   }
   const int len = length_of(p, b);
