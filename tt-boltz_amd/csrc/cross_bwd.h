@@ -102,7 +102,7 @@ template <typename T, int DP, bool BIAS, bool FEW>
 __global__ __launch_bounds__(256, (dq_waves<T, DP, BIAS, FEW>())) void xa_dq_kernel(XaParams p) {
   using M = Mma<T>;
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT, NSUB = FEW ? 1 : 2, DT = DP / 32;
-  constexpr int KS = M::row_stride(DP);
+  constexpr int KS = M::both_stride(DP);
   extern __shared__ __align__(16) char smem[];
   typedef typename M::L L;
   constexpr int PK = KT * KS, BUF = 2 * M::PARTS * PK, NBUF = buffers<T, FEW>();
@@ -290,7 +290,7 @@ constexpr int v_steps() { return DP == 128 && !Mma<T>::SPLIT ? 4 : DP / 16; }
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void xa_dkv_kernel(XaParams p) {
   using M = Mma<T>;
-  constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::row_stride(DP);
+  constexpr int RT = xa_rt(DP, __is_same(T, float)), DT = DP / 32, S = M::both_stride(DP);
   typedef typename M::L L;
   constexpr int PT = RT * S, STATS = 3 * RT * 2, NBUF = dkv_buffers<T, DP>(), BUF = 2 * M::PARTS * PT + STATS;
   constexpr bool KLDS = keys_in_lds<T, DP>();
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
   Frag<T, DP> kf, vf;
   kf.load((const T*)p.k + b * p.kb + (long)key * p.kl + hk * p.kh, p.D, h, seen, p.neg);
   vf.load((const T*)p.v + b * p.vb + (long)key * p.vl + hk * p.vh, p.D, h, seen);
-  constexpr int KLS = M::SPLIT ? DP : S;
+  constexpr int KLS = M::SPLIT ? DP : M::row_stride(DP);
   auto kl_at = [&](int s) __attribute__((always_inline)) {
     const int piece = M::SPLIT ? (2 * s + h) ^ (n & (DP / 8 - 1)) : 2 * s + h;
     return kl + (32 * wid + n) * KLS + 8 * piece;
@@ -504,7 +504,7 @@ int sum_launch(const float* part, long step, int splits, void* out0, void* out1,
 template <typename T, int DP, bool BIAS, bool FEW>
 int dq_launch(const XaParams& p, hipStream_t st) {
   constexpr int KT = FEW ? XA_KT_FEW : XA_KT;
-  const size_t tiles = (size_t)2 * KT * Mma<T>::row_stride(DP) * 2 * Mma<T>::PARTS * buffers<T, FEW>(),
+  const size_t tiles = (size_t)2 * KT * Mma<T>::both_stride(DP) * 2 * Mma<T>::PARTS * buffers<T, FEW>(),
                join = FEW ? (size_t)4 * 32 * (DP + 4) * 4 : 0, lds = tiles > join ? tiles : join;
   if (int rc = pf_reserve_lds((const void*)xa_dq_kernel<T, DP, BIAS, FEW>, lds, "xa_dq_kernel")) return rc;
   const int rt = (p.rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
@@ -529,9 +529,9 @@ int dq_type(const XaParams& p, hipStream_t st) {
 
 template <typename T, int DP, bool BIAS>
 int dkv_launch(const XaParams& p, hipStream_t st) {
-  constexpr int RT = xa_rt(DP, __is_same(T, float)), S = Mma<T>::row_stride(DP);
+  constexpr int RT = xa_rt(DP, __is_same(T, float)), S = Mma<T>::both_stride(DP);
   const size_t lds = dkv_buffers<T, DP>() * ((size_t)4 * Mma<T>::PARTS * RT * S + 3 * RT * 4) +
-                     (keys_in_lds<T, DP>() ? (size_t)2 * Mma<T>::PARTS * XA_KEYS * (Mma<T>::SPLIT ? DP : S) : 0) +
+                     (keys_in_lds<T, DP>() ? (size_t)2 * Mma<T>::PARTS * XA_KEYS * (Mma<T>::SPLIT ? DP : Mma<T>::row_stride(DP)) : 0) +
                      (v_steps<T, DP>() < DP / 16 ? (size_t)2 * XA_KEYS * (DP - 16 * v_steps<T, DP>() + 8) : 0);
   if (int rc = pf_reserve_lds((const void*)xa_dkv_kernel<T, DP, BIAS>, lds, "xa_dkv_kernel")) return rc;
   const int tiles = (p.Lk + XA_KEYS - 1) / XA_KEYS;

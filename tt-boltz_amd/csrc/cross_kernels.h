@@ -55,6 +55,8 @@ struct Mma {
   struct Packed { Op f[2]; };   // an accumulator as the right operand of a product over its 32 rows
 
   static constexpr int row_stride(int dp) { return dp + 8; }   // rows land on distinct banks (16 lanes x 16 bytes)
+  // read both ways: the same, and four rows x 32 channels of the transposing reads meet in two banks at most
+  static constexpr int both_stride(int dp) { return dp == 128 ? dp + 24 : dp + 8; }
   // only read in transposed 4 x 16 blocks: four rows x 32 channels on (nearly) distinct banks
   static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp == 64 ? 80 : dp + (SPLIT ? 8 : 32); }
 
