@@ -125,6 +125,18 @@ def test_embedding_grad_edges(gpu):
         assert torch.equal(ops.embedding_grad(do, t, 4), ops.embedding_grad(do.contiguous().clone(), t, 4))
 
 
+@pytest.mark.parametrize("C", [8, 132])
+def test_embedding_grad_padding_from_any_place(gpu, C):
+    """The last token of the table ends anywhere in a chunk, padding follows for chunks; every row is written."""
+    pad = torch.full((600,), -1, device=gpu)
+    for n in range(0, 140):
+        t = torch.cat([torch.arange(n, device=gpu) // 3, pad])
+        do, dw = torch.ones((n + 600, C), device=gpu), torch.full((50, C), torch.nan, device=gpu)
+        ws = torch.empty(ops.embedding_grad_workspace_bytes(t.numel(), 50, C), dtype=torch.uint8, device=gpu)
+        ops.launch_embedding_grad(t, do, dw, ws)
+        assert torch.equal(dw, torch.bincount(t[:n], minlength=50).float()[:, None].expand(50, C)), n
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_embedding_autograd(gpu, dtype):
     g = torch.Generator().manual_seed(5)

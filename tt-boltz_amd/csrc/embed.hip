@@ -331,7 +331,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const T* __restrict__ g
   const long i0 = chunk * p.ch, i1 = min(p.n, i0 + p.ch);
   const uint32_t none = (uint32_t)p.V;
   const bool goes_on = i0 > 0 && keys[i0 - 1] == keys[i0];   // its first run began before
-  const bool reaches = i1 < p.n && keys[i1] == keys[i1 - 1]; // its last run goes on behind
+  const bool reaches = i1 < p.n && keys[i1] == keys[i1 - 1] && keys[i1] < none;   // its last run goes on behind
   float* const part0 = parts + 2 * chunk * p.C;
   for (long c = (long)lane * N; c < p.C; c += step) {
     uint32_t cur = keys[i0];
