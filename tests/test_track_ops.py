@@ -1,5 +1,8 @@
 """The operators between tracks without a GPU: their plain forms, what they hand to the library, and what they refuse."""
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -234,3 +237,10 @@ def test_cross_attention_abi_refuses_without_launching():
         a = _lib.CrossAttnArgs(**{**back, **change})
         assert lib.pf_cross_attn_bwd(ctypes.byref(a)) == -1 and say in _err(), (change, _err())
     assert lib.pf_cross_attn_bwd(None) == -1 and "null args" in _err()
+
+
+@pytest.mark.parametrize("first", ["ops", "track_ops"])
+def test_modules_import_in_either_order(first):
+    code = (f"import importlib; m = importlib.import_module('tt_boltz_amd.{first}'); "
+            "from tt_boltz_amd import ops, track_ops; assert ops.embedding is track_ops.embedding; m.cross_attention")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=pathlib.Path(__file__).resolve().parent.parent)

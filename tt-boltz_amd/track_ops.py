@@ -22,7 +22,7 @@ from typing import Optional, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib, ops
+from . import _lib
 
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # PF_FP32 ...
 SHARED_CODE = {None: 0, "row": 1, "column": 2}                         # PF_DROP_ELEMENT ...
@@ -500,3 +500,6 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, see
     if _wants_grad(x, residual):
         return _DropoutAdd.apply(x, residual, p, seed, offset, shared)
     return _dropout_add(x, residual, p, seed, offset, shared)
+
+
+from . import ops  # noqa: E402  (which re-exports the names above, whichever of the two is imported first)
