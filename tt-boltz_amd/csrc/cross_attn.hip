@@ -4,14 +4,16 @@
 
 namespace {
 
-// Workgroups wanted: two for each of 256 CUs.
+// Workgroups wanted: two for each of 256 CUs, what most kernels' registers and LDS allow.  (dk, dv of 2 x 2048
+// keys, 4 key heads x 128 channels: 176 us, with one per CU 262; the parts of more are more to join.)
 constexpr long WANT = 512;
 
 struct Split { int splits, per; };
 
-// `tiles` of one axis split so that `base` workgroups become WANT, at least `least` tiles each
+// `tiles` of one axis split so that `base` workgroups become up to WANT (a few more than that wait for all
+// the others: fp32 dk, dv of 184 workgroups 51 us in 3 parts, 42 in 2), at least `least` tiles each
 Split split_of(long base, long tiles, long least) {
-  long s = base > 0 ? (WANT + base - 1) / base : 1;
+  long s = base > 0 ? WANT / base : 1;
   if (s > tiles / least) s = tiles / least;
   if (s > 64) s = 64;
   if (s < 1) s = 1;
@@ -73,7 +75,7 @@ XaParams params_of(const pf_cross_attn_args* a) {
 // the split over key tiles of the forward and the dq kernel (an fp32 tile is worth several of 16 bits)
 Split key_split(const XaParams& p, int dtype) {
   const long rows = p.few ? 32 : 128, kt = p.few ? XA_KT_FEW : XA_KT;
-  return split_of((p.rows + rows - 1) / rows * p.B * p.Hk, (p.Lk + kt - 1) / kt, p.few ? 1 : dtype == PF_FP32 ? 2 : 4);
+  return split_of((p.rows + rows - 1) / rows * p.B * p.Hk, (p.Lk + kt - 1) / kt, p.few ? 1 : dtype == PF_FP32 ? 2 : 3);
 }
 // the split over row tiles of the dk, dv kernel
 Split row_split(const XaParams& p, int dtype) {

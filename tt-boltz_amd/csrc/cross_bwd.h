@@ -429,8 +429,8 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
           for (int k = 0; k < 16; ++k) pr[k] = seen ? pr[k] : 0.f;
         }
         const typename M::Packed pv[1] = {M::pack(pr)};
-                M::template outer<DT, 1>(gs + 32 * u * S, PT, S, lane, pv, dv);
-        #pragma unroll
+        M::template outer<DT, 1>(gs + 32 * u * S, PT, S, lane, pv, dv);
+#pragma unroll
         for (int run = 0; run < 4; ++run) {
           const f32x4 dl = *reinterpret_cast<const f32x4*>(st + 2 * RT + 32 * u + 8 * run + 4 * h);
 #pragma unroll
@@ -439,11 +439,11 @@ __global__ __launch_bounds__(256, DP == 128 && __is_same(T, float) ? 1 : 2) void
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
           dp = M::mma(M::load(gs + at + 16 * s, PT), s < VST ? vf.f[s] : M::load(vl_row + 16 * (s - VST), 0), dp);
-        #pragma unroll
+#pragma unroll
         for (int k = 0; k < 16; ++k) dp[k] = pr[k] * (SCALED<T> ? dp[k] * ds_f : dp[k]);
         const typename M::Packed pd[1] = {M::pack(dp)};
         M::template outer<DT, 1>(qs + 32 * u * S, PT, S, lane, pd, dk);
-              }
+      }
     }
     if constexpr (NBUF == 1) __syncthreads();
     if (t + 1 < t1) store_tile(t + 1);
