@@ -50,37 +50,28 @@ PF_DEV void drop_store(const T* r, T* out, uint64_t e, const float (&y)[N]) {
   }
 }
 
-// One mask value per element.  N elements a step (16 bytes, or 1 where a pointer or the size allows
-// no more: N = 1 makes a whole counter for each element); U steps a thread in flight, a grid's width
-// apart.
-template <typename T, int N, int U>
+// One mask value per element.  N elements a thread (16 bytes, or 1 where a pointer or the size allows no
+// more: N = 1 makes a whole counter for each element).
+template <typename T, int N>
 __global__ __launch_bounds__(256) void dropout_elem_kernel(const T* __restrict__ x, const T* __restrict__ r,
                                                            T* __restrict__ out, DropShape p) {
+  const uint64_t e = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * N;
+  if (e >= p.total) return;
   const uint64_t seed = p.seed_at ? *p.seed_at : p.seed;
-  const uint64_t e0 = ((uint64_t)blockIdx.x * (256 * U) + threadIdx.x) * N;
-  float v[U][N];
+  float v[N];
+  load_elems<T, N>(x + e, v);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t e = e0 + (uint64_t)u * 256 * N;
-    if (e < p.total) load_elems<T, N>(x + e, v[u]);
-  }
+  for (int q = 0; q < (N + 3) / 4; ++q) {
+    const Words w = philox(seed, e / 4 + q, p.offset);
+    if constexpr (N == 1) {
+      const uint32_t c = (uint32_t)e & 3, lo = c & 1 ? w.w[1] : w.w[0], hi = c & 1 ? w.w[3] : w.w[2];
+      v[0] = (c & 2 ? hi : lo) >= p.threshold ? v[0] * p.scale : 0.f;
+    } else {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t e = e0 + (uint64_t)u * 256 * N;
-    if (e >= p.total) break;
-#pragma unroll
-    for (int q = 0; q < (N + 3) / 4; ++q) {
-      const Words w = philox(seed, e / 4 + q, p.offset);
-      if constexpr (N == 1) {
-        const uint32_t c = (uint32_t)e & 3, lo = c & 1 ? w.w[1] : w.w[0], hi = c & 1 ? w.w[3] : w.w[2];
-        v[u][0] = (c & 2 ? hi : lo) >= p.threshold ? v[u][0] * p.scale : 0.f;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][4 * q + i] = w.w[i] >= p.threshold ? v[u][4 * q + i] * p.scale : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) v[4 * q + i] = w.w[i] >= p.threshold ? v[4 * q + i] * p.scale : 0.f;
     }
-    drop_store<T, N>(r, out, e, v[u]);
   }
+  drop_store<T, N>(r, out, e, v);
 }
 
 // One mask value per (batch, row): blockIdx.y counts them (in steps of gridDim.y), so the generator
@@ -160,15 +151,14 @@ int launch(const void* xv, const void* rv, void* ov, const DropShape& p, int sha
   constexpr unsigned MOST_Y = 65535;
   const uint64_t len = (uint64_t)p.cols * p.channels;
   if (shared == PF_DROP_ELEMENT) {
-    constexpr int U = 2;
-    dropout_elem_kernel<T, N, U><<<blocks_of(p.total, 256 * U * N), 256, 0, st>>>(x, r, out, p);
+    dropout_elem_kernel<T, N><<<blocks_of(p.total, 256 * N), 256, 0, st>>>(x, r, out, p);
   } else if (shared == PF_DROP_ROW) {
-    constexpr int U = 4;
+    constexpr int U = 2;
     const uint64_t groups = p.total / len;
     dropout_row_kernel<T, N, U><<<dim3(blocks_of(len, 256 * U * N), (unsigned)(groups < MOST_Y ? groups : MOST_Y)), 256, 0,
                                   st>>>(x, r, out, p);
   } else {
-    constexpr int ROWS = 4;
+    constexpr int ROWS = 2;
     const uint64_t steps = p.total / len / p.rows * ((p.rows + ROWS - 1) / ROWS);
     dropout_col_kernel<T, N, ROWS><<<dim3(blocks_of(len, 256 * N), (unsigned)(steps < MOST_Y ? steps : MOST_Y)), 256, 0,
                                      st>>>(x, r, out, p);

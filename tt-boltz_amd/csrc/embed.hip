@@ -18,11 +18,13 @@
 namespace {
 
 // ------------------------------------------------------------------------------ forward
-// A group of TPR lanes (a power of two) copies U rows; N elements (16 bytes, or 1) a load.
+constexpr int LOOKUP_ROWS = 2;
+
+// A group of lanes (a power of two) copies LOOKUP_ROWS rows; N elements (16 bytes, or 1) a load.
 template <typename T, int N, typename I>
 __global__ __launch_bounds__(256) void embed_kernel(const I* __restrict__ t, const T* __restrict__ w, long ldw,
                                                     T* __restrict__ out, long n, long V, long C, float scale, int tpr_log2) {
-  constexpr int U = 4;
+  constexpr int U = LOOKUP_ROWS;
   const int tpr = 1 << tpr_log2, groups = 256 >> tpr_log2;
   const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x >> tpr_log2;
   const long i0 = (long)blockIdx.x * (groups * U) + group;
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const T* __restrict__ g
   }
   // part 1: a group of lanes streams the CH tokens of a chunk in their sorted order, U rows in flight, and
   // writes a sum where the token changes
-  constexpr int U = 8;
+  constexpr int U = 4;
   const long chunk = (long)blockIdx.x * groups + group;
   if (chunk >= p.chunks) return;
   const long i0 = chunk * p.ch, i1 = min(p.n, i0 + p.ch);
@@ -517,8 +519,8 @@ GradLayout grad_layout(long n, long V, long C) {
   // chunks of 32 tokens while that gives the chip no more than 2^18 lanes, longer ones (fewer crossed
   // borders) behind that; C / 4 lanes a row at most
   const int lanes = C >= 1024 ? 256 : 1 << log2_at_least((C + 3) / 4);
-  l.ch = 32;
-  while (l.ch < 256 && n / l.ch * lanes > (1l << 18)) l.ch *= 2;
+  l.ch = n / 16 * lanes <= (1l << 16) ? 16 : 32;
+  while (l.ch < 256 && n / l.ch > 8192) l.ch *= 2;
   l.chunks = (n + l.ch - 1) / l.ch;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
   const size_t list = up((size_t)n * 4);
@@ -544,7 +546,7 @@ template <typename T, int N>
 int embed_launch(const void* t, int index64, const T* w, long ldw, T* out, long n, long V, long C, float scale,
                  hipStream_t st) {
   const int units = (int)((C + N - 1) / N), tpr_log2 = units >= 256 ? 8 : log2_at_least(units);
-  const long per = 4l * (256 >> tpr_log2);
+  const long per = (long)LOOKUP_ROWS * (256 >> tpr_log2);
   const long grid_l = (n + per - 1) / per;
   if (grid_l >> 24)   // a launch holds fewer than 2^32 threads
     return pf_fail(PF_E_INVALID, "pf_embedding_fwd: too many rows (n=%ld C=%ld)", n, C);
