@@ -20,6 +20,9 @@ Contents
                     weighted averaging, MSA layer, input embedding).
 ``diffusion_ref``   fp32 restatement of the pair side of the diffusion conditioning
                     (PairwiseConditioning, the token-transformer pair bias).
+``track_ref``       64-bit forms of the operators between tracks (cross attention, table
+                    lookup and its gradient, residual dropout) and the error bounds their
+                    roundings allow.
 ``brute``           scalar-loop restatements for tiny sizes (N <= 8), used by the
                     tests to pin ``pairformer_ref`` independently of torch's
                     einsum / matmul / softmax.

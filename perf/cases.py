@@ -12,7 +12,7 @@ A case is a dict of plain values.  Its ``op`` names the entry point a program ca
 * ``msa``         ``MSAModule``: one block of the MSA stack
 * ``diffusion``   ``DiffusionPairConditioning``: the pair side of the diffusion conditioning
 
-Inference only: the framework has no backward pass.  Sizes are token counts ``n`` (and MSA
+Inference: none of these calls has a backward pass.  Sizes are token counts ``n`` (and MSA
 depths); ``tail`` tokens at the end are masked.  ``operand`` is the 16-bit matrix operand type
 and ``fast`` the block-fp8 mode.
 """

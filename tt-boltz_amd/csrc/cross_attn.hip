@@ -72,7 +72,9 @@ XaParams params_of(const pf_cross_attn_args* a) {
   return p;
 }
 
-// the split over key tiles of the forward and the dq kernel (an fp32 tile is worth several of 16 bits)
+// the split over key tiles of the forward and the dq kernel.  Three tiles of 16 bits a part at least: 2 x 512
+// x 765, 16 heads, four parts of 3 tiles 17.4 us, three of 4 20.6; 64 rows x 8 heads over 8192 keys 14.9 in
+// 32 or 42 parts, 17.3 in 64.  An fp32 tile is worth several (2, 1 and 4 within a microsecond of each other).
 Split key_split(const XaParams& p, int dtype) {
   const long rows = p.few ? 32 : 128, kt = p.few ? XA_KT_FEW : XA_KT;
   return split_of((p.rows + rows - 1) / rows * p.B * p.Hk, (p.Lk + kt - 1) / kt, p.few ? 1 : dtype == PF_FP32 ? 2 : 3);

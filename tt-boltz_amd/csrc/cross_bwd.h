@@ -7,6 +7,13 @@
 // fp16: dS and P are products' operands and far smaller than 1, where fp16 has few bits left (below
 // 2^-14) or none (2^-25).  P is taken 2^15 times larger, and dS by the power of two that brings its
 // bound max|do_i| max|v_j| 2 to 2^14 or less; both factors are divided out of the fp32 sums.
+//
+// Measured (one MI355X, us a launch): 2 x 2048 queries x 2048 keys of which about three quarters are seen, 16
+// heads over 4, 128 channels, bf16: dq 115, dk and dv 176 and 12.5 for the sum of their four splits, delta 10
+// (50 MB).  2 x 512 x 765, 16 heads x 24, fp16 with a bias whose gradient is wanted: dq 31 (50 MB of bias and
+// dS), dk and dv 26, delta 5, sums 4.5 each.  fp32, 384 x 2900 x 8 heads x 48: dq 36, dk and dv 43, delta 4,
+// sums 5 each.  Both large kernels hold two waves per SIMD (accumulators and operands fill the registers),
+// which leaves LDS reads and MFMAs of one wave waiting for each other part of the time.
 #pragma once
 #include "cross_kernels.h"
 

@@ -11,6 +11,13 @@
 // from LDS in the accumulators' key order.  The dk, dv kernel forms S = Q K^T: its lanes hold keys.
 //
 // Heads that share a key head are rows of one tile, so keys and values are read once for them.
+//
+// Measured (one MI355X, us a launch).  Forward: 4 x 2048 queries x 4096 keys, 16 heads x 64 channels, bf16 165
+// to 190 (830 to 720 TFLOP/s; 4 x 32 channels 148, 128 channels 348 = 790 TFLOP/s); beside the MFMAs each
+// score costs an exponential, a rounding and the sum, so matrix and vector units are both busy and the clock
+// falls to what power allows.  512 windows of 32 x 128, 4 heads x 32 with bias 18.5 (75 MB: 4.1 TB/s, 15.5 at
+// a copy's rate).  8 x 1 query x 1536 keys, 16 heads over 4: 7.0 and 3.3 for the join, both latency.  fp32,
+// 384 x 2900 x 8 heads x 48: 29 and 5 (six products for one).
 #pragma once
 #include "cross_attn.h"
 
@@ -56,6 +63,7 @@ struct Mma {
 
   static constexpr int row_stride(int dp) { return dp + 8; }   // rows land on distinct banks (16 lanes x 16 bytes)
   // read both ways: the same, and four rows x 32 channels of the transposing reads meet in two banks at most
+  // (2 x 2048 x 2048, 16 heads over 4, 128 channels: dk, dv 176 us, with dp + 8 185; dq 115 and 118)
   static constexpr int both_stride(int dp) { return dp == 128 ? dp + 24 : dp + 8; }
   // only read in transposed 4 x 16 blocks: four rows x 32 channels on (nearly) distinct banks
   static constexpr int col_stride(int dp) { return dp == 32 ? 32 : dp == 64 ? 80 : dp + (SPLIT ? 8 : 32); }
@@ -337,7 +345,7 @@ PF_DEV void load_keys(Stage<T, DP, KT>& s, const T* base, int stride, int D, int
 }
 
 // Workgroup w runs on XCD w % 8: neighbouring ids go to one XCD, so the workgroups of a (batch, key head)
-// share its keys and values in one L2.
+// share its keys and values in one L2 (4 x 2048 x 4096: 167 us, in launch order 178; windows 13.4 and 16.7).
 PF_DEV int xcd_remap(int w, int total) {
   const int x = w % 8, q = total / 8, rem = total % 8;
   return x * q + min(x, rem) + w / 8;
@@ -418,15 +426,18 @@ PF_DEV void store4(T* p, const float (&x)[4]) {
 }
 
 // ------------------------------------------------------------------------------ forward
-// FEW = false: every wave over the tile's 64 keys with R tiles of 32 rows.  FEW = true (at most 32 rows): the waves share one
-// 32-row tile and take 32 of the tile's 128 keys each; their results are joined through LDS.
+// FEW = false: every wave over the tile's 64 keys with R tiles of 32 rows.  FEW = true (at most 32 rows): the
+// waves share one 32-row tile and take 32 of the tile's 128 keys each; their results are joined through LDS
+// (512 windows of 32 x 128: 13.5 us, as rows of a 128-row tile 15.5; 8 requests of one query: 10.4 and 12.0).
 //
-// LDS buffers of a tile: two, so that a tile needs one barrier, or one where the tiles are large and more
-// workgroups per CU are worth more (single rows stream keys at memory's rate).
+// LDS buffers of a tile: two, so that a tile needs one barrier (128 channels: 85 us, with one buffer 129), or
+// one where the tiles are large and more workgroups per CU are worth more (single rows stream keys at memory's
+// rate; fp32's three parts).
 template <typename T, bool FEW>
 constexpr int buffers() { return FEW || __is_same(T, float) ? 1 : 2; }
 
-// Waves per SIMD that the forward kernel's registers are kept to.
+// Waves per SIMD that the forward kernel's registers are kept to: the most that holds its accumulators and
+// the tile on its way without spilling.
 template <typename T, int DP, bool BIAS, bool FEW, int R, bool WHOLE>
 constexpr int fwd_waves() {
   if (WHOLE && DP <= 64) return FEW && DP == 32 ? 3 : 2;
@@ -437,7 +448,7 @@ constexpr int fwd_waves() {
 
 // WHOLE (16-bit types): P enters the product with the values to fp32's accuracy.  A bias's gradient is
 // dS = P (dP - delta) itself, fp32 as a rule, and delta = do . o of an o made from rounded P would leave it
-// with 2^-9 or 2^-12 of delta.
+// with 2^-9 or 2^-12 of delta.  (2 x 512 x 765, 16 heads x 24, fp16: 17.6 us.)
 template <typename T, int DP, bool BIAS, bool FEW, int R, bool WHOLE>
 __global__ __launch_bounds__(256, (fwd_waves<T, DP, BIAS, FEW, R, WHOLE>())) void xa_fwd_kernel(XaParams p) {
   using M = Mma<T>;
