@@ -353,6 +353,16 @@ def test_cross_attention(gpu, B, Lq, Lk, H, Hk, D, bias, hide, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias,hide", [(None, "both"), ("full", "lens")])
+@pytest.mark.parametrize("Lq,Lk,H,Hk,D", [(1, 2300, 2, 1, 8), (2, 5000, 2, 2, 24), (1, 9000, 1, 1, 128), (40, 4200, 2, 2, 64), (35, 8200, 1, 1, 104)])
+def test_cross_attention_joins_of_many_parts(gpu, Lq, Lk, H, Hk, D, bias, hide, dtype):
+    """Few queries over long keys, and a batch element whose later parts see nothing."""
+    c, do = inputs(Lk + D, dtype, 2, Lq, Lk, H, Hk, D, bias, hide)
+    c["k_lens"][1] = 150
+    check_cross(c, do, gpu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.7])
 def test_cross_attention_scales(gpu, dtype, scale):
     c, do = inputs(3, dtype, 2, 40, 90, 2, 2, 32, "full", "mask")

@@ -144,7 +144,7 @@ def test_abi_refuses_without_launching():
     ok = dict(B=1, I=1, J=1, C=8, dtype=0, shared=0, p=0.5, x=d, out=d)
     for change, say in ((dict(dtype=3), "dtype"), (dict(shared=3), "sharing"), (dict(p=1.5), "p must"), (dict(p=float("nan")), "p must"),
                         (dict(B=-1), "bad shape"), (dict(C=1 << 33), "bad shape"), (dict(B=1 << 40, C=1 << 30), "2\\^32"),
-                        (dict(x=None), "null"), (dict(out=None), "null")):
+                        (dict(x=None), "null"), (dict(out=None), "null"), (dict(C=1 << 16, J=1 << 16, x=d + 4), "aligned")):
         a = _lib.DropoutArgs(**{**ok, **change})
         assert lib.pf_dropout_add_fwd(ctypes.byref(a)) == -1
         import re
@@ -233,6 +233,7 @@ def test_cross_attention_abi_refuses_without_launching():
                         (dict(dbias=d, dbias_B=2, dbias_H=4), "does not belong"), (dict(dbias_B=2, dbias_H=4), "do not agree"),
                         (dict(bias=d, dbias=d, dbias_B=1, dbias_H=4, dq=None), "comes with dq"),
                         (dict(bias=d, dbias=d, dbias_B=3, dbias_H=4), "does not belong"), (dict(workspace_bytes=16), "workspace too small"),
+                        (dict(bias=d, dbias=d, dbias_B=1, dbias_H=4, Lq=65535, Lk=65537), "too large"),
                         (dict(dq=d + 4), "aligned"), (dict(Lq=0), "no queries")):
         a = _lib.CrossAttnArgs(**{**back, **change})
         assert lib.pf_cross_attn_bwd(ctypes.byref(a)) == -1 and say in _err(), (change, _err())

@@ -198,7 +198,7 @@ extern "C" int pf_cross_attn_bwd(const pf_cross_attn_args* a) {
     return pf_fail(PF_E_INVALID, "%s: gradients and workspace must be 16-byte aligned", fn);
   XaParams p = params_of(a);
   if (!grid_fits(p, true)) return pf_fail(PF_E_INVALID, "%s: too large (B=%d Lq=%d Lk=%d H=%d)", fn, a->B, a->Lq, a->Lk, a->H);
-  if (a->dbias && (((long)a->Lq * a->Lk) >> 32 || (long)a->dbias_B * a->dbias_H > 65535))
+  if (a->dbias && ((long)a->Lq * a->Lk > (1l << 32) - 256 || (long)a->dbias_B * a->dbias_H > 65535))
     return pf_fail(PF_E_INVALID, "%s: bias gradient too large (Lq=%d Lk=%d B=%d H=%d)", fn, a->Lq, a->Lk, a->dbias_B, a->dbias_H);
   const BwdLayout l = bwd_layout(a, p);
   if (!a->workspace || a->workspace_bytes < (size_t)l.bytes)

@@ -178,6 +178,8 @@ int launch_type(const void* x, const void* r, void* out, const DropShape& p, int
   constexpr int N = Vec16<T>::N;
   const uint64_t inner = shared == PF_DROP_ELEMENT ? p.total : shared == PF_DROP_ROW ? (uint64_t)p.cols * p.channels : p.channels;
   const bool wide = pf_aligned16(x) && pf_aligned16(r) && pf_aligned16(out) && inner % N == 0;
+  if (!wide && p.total > (1ull << 32) - 256)   // a launch holds fewer than 2^32 threads
+    return pf_fail(PF_E_INVALID, "pf_dropout_add_fwd: 2^32 elements need 16-byte aligned tensors");
   return wide ? launch<T, N>(x, r, out, p, shared, st) : launch<T, 1>(x, r, out, p, shared, st);
 }
 
