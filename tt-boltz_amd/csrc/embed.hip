@@ -16,7 +16,7 @@
 //
 // Memory's rate bounds all but the smallest.  Measured (one MI355X): lookup of 16384 rows of 2048 bf16 out of
 // 32000 17 to 21 us (134 MB, rows that come again from cache), of 524288 x 64 fp32 out of 33 22.5 (134 MB
-// written: 6.0 TB/s).  Gradient of the latter: sums 23 us (134 MB read), join 9.5, sort 20; of 16384 x 2048 bf16
+// written: 6.0 TB/s).  Gradient of the latter: sums 23 us (134 MB read), join 9.5, sort 16; of 16384 x 2048 bf16
 // in 128000 rows: sums and zeros 106 to 114 (591 MB, of which the 524 written alone take a fill 76), join 8,
 // sort 27 for its two digits.  Up to 4096 tokens 10 to 40 us, the launches' and the sort's latency.
 #include "pf_elem.h"
@@ -202,15 +202,26 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const void* __restrict_
 }
 
 // counts [digit][workgroup]: a wave per digit replaces them by the sums of the workgroups before, and
-// leaves the digit's total behind them (totals[digit]).
+// leaves the digit's total behind them (totals[digit]).  A lane has U consecutive workgroups.
 __global__ __launch_bounds__(64) void sort_scan_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int blocks) {
+  constexpr int U = 8;
   uint32_t* const c = counts + (long)blockIdx.x * blocks;
   const int lane = threadIdx.x;
   uint32_t before = 0;
-  for (int b0 = 0; b0 < blocks; b0 += 64) {
-    const int b = b0 + lane;
-    const uint32_t x = b < blocks ? c[b] : 0, upto = wave_scan(x, lane);
-    if (b < blocks) c[b] = before + upto - x;
+  for (int b0 = 0; b0 < blocks; b0 += 64 * U) {
+    const int b = b0 + U * lane;
+    uint32_t x[U], sum = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = b + u < blocks ? c[b + u] : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum += x[u];
+    const uint32_t upto = wave_scan(sum, lane);
+    uint32_t at = before + upto - sum;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (b + u < blocks) c[b + u] = at;
+      at += x[u];
+    }
     before += __shfl(upto, 63);
   }
   if (lane == 0) totals[blockIdx.x] = before;
