@@ -168,7 +168,7 @@ def test_embedding_grad_by_differences(gpu):
 
 # ------------------------------------------------------------------------------ dropout
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape,shared", [((1,), None), ((3, 5), None), ((2, 100, 16), None), ((4099,), None), ((2, 1, 24), "row"),
+@pytest.mark.parametrize("shape,shared", [((1,), None), ((3, 5), None), ((2, 100, 16), None), ((4099,), None), ((8,), None), ((7,), None), ((2047, 5), None), ((8193,), None), ((3, 1367), None), ((2, 1, 24), "row"),
                                           ((2, 5, 7, 16), "row"), ((3, 6, 6, 5), "row"), ((2, 5, 7, 16), "column"),
                                           ((9, 4, 3), "column"), ((2, 2, 3, 10, 8), "column")])
 def test_dropout_add(gpu, dtype, shape, shared):

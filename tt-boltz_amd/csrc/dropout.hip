@@ -54,27 +54,31 @@ PF_DEV void drop_store(const T* r, T* out, uint64_t e, const float (&y)[N]) {
   }
 }
 
-// One mask value per element.  N elements a thread (16 bytes, or 1 where a pointer or the size allows no
-// more: N = 1 makes a whole counter for each element).  A second step a thread costs 31.5 us for 29, the
-// smallest sizes (64 K elements) 3.0 for 2.4.
+// One mask value per element.  N elements a thread (16 bytes, or 1 where a pointer allows no more: N = 1
+// makes a whole counter for each element, as do the last few of a number that N does not divide).  A second
+// step a thread costs 31.5 us for 29, the smallest sizes (64 K elements) 3.0 for 2.4.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void dropout_elem_kernel(const T* __restrict__ x, const T* __restrict__ r,
                                                            T* __restrict__ out, DropShape p) {
   const uint64_t e = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * N;
   if (e >= p.total) return;
   const uint64_t seed = p.seed_at ? *p.seed_at : p.seed;
+  if (N == 1 || e + N > p.total) {
+    for (uint64_t k = e; k < p.total && k < e + N; ++k) {
+      const Words w = philox(seed, k / 4, p.offset);
+      const uint32_t c = (uint32_t)k & 3, lo = c & 1 ? w.w[1] : w.w[0], hi = c & 1 ? w.w[3] : w.w[2];
+      const float y[1] = {(c & 2 ? hi : lo) >= p.threshold ? (float)x[k] * p.scale : 0.f};
+      drop_store<T, 1>(r, out, k, y);
+    }
+    return;
+  }
   float v[N];
   load_elems<T, N>(x + e, v);
 #pragma unroll
-  for (int q = 0; q < (N + 3) / 4; ++q) {
+  for (int q = 0; q < N / 4; ++q) {
     const Words w = philox(seed, e / 4 + q, p.offset);
-    if constexpr (N == 1) {
-      const uint32_t c = (uint32_t)e & 3, lo = c & 1 ? w.w[1] : w.w[0], hi = c & 1 ? w.w[3] : w.w[2];
-      v[0] = (c & 2 ? hi : lo) >= p.threshold ? v[0] * p.scale : 0.f;
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * q + i] = w.w[i] >= p.threshold ? v[4 * q + i] * p.scale : 0.f;
-    }
+    for (int i = 0; i < 4; ++i) v[4 * q + i] = w.w[i] >= p.threshold ? v[4 * q + i] * p.scale : 0.f;
   }
   drop_store<T, N>(r, out, e, v);
 }
@@ -176,7 +180,7 @@ int launch(const void* xv, const void* rv, void* ov, const DropShape& p, int sha
 template <typename T>
 int launch_type(const void* x, const void* r, void* out, const DropShape& p, int shared, hipStream_t st) {
   constexpr int N = Vec16<T>::N;
-  const uint64_t inner = shared == PF_DROP_ELEMENT ? p.total : shared == PF_DROP_ROW ? (uint64_t)p.cols * p.channels : p.channels;
+  const uint64_t inner = shared == PF_DROP_ELEMENT ? N : shared == PF_DROP_ROW ? (uint64_t)p.cols * p.channels : p.channels;
   const bool wide = pf_aligned16(x) && pf_aligned16(r) && pf_aligned16(out) && inner % N == 0;
   if (!wide && p.total > (1ull << 32) - 256)   // a launch holds fewer than 2^32 threads
     return pf_fail(PF_E_INVALID, "pf_dropout_add_fwd: 2^32 elements need 16-byte aligned tensors");
