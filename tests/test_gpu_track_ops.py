@@ -51,7 +51,7 @@ def tokens(g, dist, n, V):
 
 # ------------------------------------------------------------------------------ lookup
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,V,C", [(1, 1, 1), (1, 7, 128), (5, 33, 64), (257, 100, 24), (100, 513, 130), (33, 40, 2056),
+@pytest.mark.parametrize("n,V,C", [(300, 50, 12), (70, 9, 1100), (1, 1, 1), (1, 7, 128), (5, 33, 64), (257, 100, 24), (100, 513, 130), (33, 40, 2056),
                                    (1000, 3, 8)])
 def test_embedding(gpu, dtype, n, V, C):
     g = torch.Generator().manual_seed(n + V + C)
@@ -89,7 +89,7 @@ def test_embedding_offsets_past_32_bits(gpu):
 # ------------------------------------------------------------------------------ its gradient
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,V,C,dist", [
-    (1, 1, 1, "one"), (1, 5, 8, "uniform"), (64, 1, 16, "one"), (65, 3, 16, "one"), (129, 1, 7, "one"), (63, 100, 128, "uniform"),
+    (2000, 300, 12, "uniform"), (900, 7, 1100, "uniform"), (1, 1, 1, "one"), (1, 5, 8, "uniform"), (64, 1, 16, "one"), (65, 3, 16, "one"), (129, 1, 7, "one"), (63, 100, 128, "uniform"),
     (1024, 33, 64, "uniform"), (1025, 33, 65, "few"), (3000, 700, 24, "uniform"), (4097, 200, 132, "sorted"),
     (2500, 600, 16, "few"), (700, 40, 2056, "few"), (5000, 300000, 8, "uniform"), (300, 50, 1100, "one")])
 def test_embedding_grad(gpu, dtype, n, V, C, dist):
@@ -168,7 +168,9 @@ def test_embedding_grad_by_differences(gpu):
 
 # ------------------------------------------------------------------------------ dropout
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape,shared", [((1,), None), ((3, 5), None), ((2, 100, 16), None), ((4099,), None), ((8,), None), ((7,), None), ((2047, 5), None), ((8193,), None), ((3, 1367), None), ((2, 1, 24), "row"),
+@pytest.mark.parametrize("shape,shared", [((1,), None), ((3, 5), None), ((2, 100, 16), None), ((4099,), None), ((2, 1, 24), "row"),
+                                          ((8,), None), ((7,), None), ((2047, 5), None), ((8193,), None), ((3, 1367), None),
+                                          ((2, 5, 7, 12), "row"), ((2, 6, 5, 12), "column"), ((1, 9, 301, 132), "column"),
                                           ((2, 5, 7, 16), "row"), ((3, 6, 6, 5), "row"), ((2, 5, 7, 16), "column"),
                                           ((9, 4, 3), "column"), ((2, 2, 3, 10, 8), "column")])
 def test_dropout_add(gpu, dtype, shape, shared):

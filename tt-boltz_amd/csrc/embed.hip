@@ -586,6 +586,11 @@ int embed_type(const void* t, int index64, const void* w, long ldw, void* out, l
   constexpr int N = Vec16<T>::N;
   if (C % N == 0 && ldw % N == 0 && pf_aligned16(w) && pf_aligned16(out))
     return embed_launch<T, N>(t, index64, (const T*)w, ldw, (T*)out, n, V, C, scale, st);
+  // 8 bytes of 16-bit types: 16384 x 2044 bf16 out of 32000 22 us, one element a lane 31
+  if constexpr (N == 8) {
+    if (C % 4 == 0 && ldw % 4 == 0 && pf_aligned16(w) && pf_aligned16(out))
+      return embed_launch<T, 4>(t, index64, (const T*)w, ldw, (T*)out, n, V, C, scale, st);
+  }
   return embed_launch<T, 1>(t, index64, (const T*)w, ldw, (T*)out, n, V, C, scale, st);
 }
 
@@ -650,6 +655,10 @@ int grad_type(const void* g, const uint32_t* keys, const uint32_t* pos, void* dw
   constexpr int N = Vec16<T>::N;
   if (C % N == 0 && pf_aligned16(g) && pf_aligned16(dw))
     return grad_sums<T, N>((const T*)g, keys, pos, (T*)dw, ws, l, n, V, C, scale, st);
+  if constexpr (N == 8) {   // (the same sizes: 71 us and 166)
+    if (C % 4 == 0 && pf_aligned16(g) && pf_aligned16(dw))
+      return grad_sums<T, 4>((const T*)g, keys, pos, (T*)dw, ws, l, n, V, C, scale, st);
+  }
   return grad_sums<T, 1>((const T*)g, keys, pos, (T*)dw, ws, l, n, V, C, scale, st);
 }
 

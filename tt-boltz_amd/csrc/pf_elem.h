@@ -20,13 +20,14 @@ struct Vec16 {
   typedef T type __attribute__((ext_vector_type(N)));
 };
 
-// N consecutive elements as floats; N * sizeof(T) is 16 (aligned) or N = 1
+// N consecutive elements as floats; N is 1, or 4 or 8 of at most 16 bytes, aligned to their size
 template <typename T, int N>
 PF_DEV void load_elems(const T* p, float (&x)[N]) {
   if constexpr (N == 1) {
     x[0] = (float)p[0];
   } else {
-    const auto v = *reinterpret_cast<const typename Vec16<T>::type*>(p);
+    typedef T vec_t __attribute__((ext_vector_type(N)));
+    const vec_t v = *reinterpret_cast<const vec_t*>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = (float)v[i];
   }
@@ -37,10 +38,11 @@ PF_DEV void store_elems(T* p, const float (&x)[N]) {
   if constexpr (N == 1) {
     p[0] = (T)x[0];
   } else {
-    typename Vec16<T>::type v;
+    typedef T vec_t __attribute__((ext_vector_type(N)));
+    vec_t v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
-    *reinterpret_cast<typename Vec16<T>::type*>(p) = v;
+    *reinterpret_cast<vec_t*>(p) = v;
   }
 }
 
