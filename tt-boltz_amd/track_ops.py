@@ -344,7 +344,8 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         index, = ctx.saved_tensors
-        return None, embedding_grad(grad, index, ctx.rows, ctx.scale), None
+        again = grad.requires_grad and torch.is_grad_enabled()   # a gradient of this gradient is wanted
+        return None, (embedding_grad if again else _embedding_grad)(grad, index, ctx.rows, ctx.scale), None
 
 
 def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
@@ -458,7 +459,8 @@ class _DropoutAdd(torch.autograd.Function):
         p, seed, offset, shared = ctx.args
         if seed is None:
             seed, = ctx.saved_tensors
-        dx = dropout_add(grad, None, p, seed, offset, shared) if ctx.needs_input_grad[0] else None
+        again = grad.requires_grad and torch.is_grad_enabled()   # a gradient of this gradient is wanted
+        dx = (dropout_add if again else _dropout_add)(grad, None, p, seed, offset, shared) if ctx.needs_input_grad[0] else None
         return dx, grad if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
